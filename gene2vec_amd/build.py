@@ -30,6 +30,11 @@ ARCH = "gfx950"
 # must stay a diamond for the loop head to wait with vmcnt(#row instructions)
 # instead of vmcnt(0) (g2v_sgns_atomic.hip; tests/test_kernel_isa.py)
 SGNS_KERNEL_FLAGS = ("-mllvm", "-structurizecfg-skip-uniform-regions=true")
+# no packed fp32 arithmetic (v_pk_add / mul / fma_f32): the compiler forms it
+# from ordinary float code, and some of its forms have given wrong results on
+# MI355X.  Every device unit; the host pass warns that it does not know the
+# feature, which is harmless
+DEVICE_FLAGS = ("-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops")
 # the sources that determine k_sgns_atomic's code (bench.py accepts a PMC
 # traffic profile only when it was measured on this exact kernel code AND the
 # same launch layout: grid and stripe tiers, recorded beside the hash)
@@ -94,7 +99,8 @@ def build(force: bool = False, verbose: bool = False, ablations: bool = False,
     # the objects' compile flags are part of their key: a stamp in
     # the object directory; another flag set rebuilds every object there
     stamp = os.path.join(objdir, "flags.stamp")
-    key = " ".join(flags + ["|"] + list(SGNS_KERNEL_FLAGS) + list(kernel_flags))
+    key = " ".join(flags + ["|"] + list(DEVICE_FLAGS) + list(SGNS_KERNEL_FLAGS)
+                   + list(kernel_flags))
     old_key = open(stamp).read() if os.path.exists(stamp) else None
     if old_key is not None and old_key != key:
         force = True
@@ -111,7 +117,8 @@ def build(force: bool = False, verbose: bool = False, ablations: bool = False,
                 and all(os.path.getmtime(d) <= os.path.getmtime(objs[i]) for d in deps)):
             return ""
         kf = (list(SGNS_KERNEL_FLAGS) + list(kernel_flags)) if src == "g2v_sgns_atomic.hip" else []
-        cmd = [hipcc(), *flags, *kf, *defs, "-c", os.path.join(CSRC, src), "-o", objs[i]]
+        df = DEVICE_FLAGS if src.endswith(".hip") else ()
+        cmd = [hipcc(), *flags, *df, *kf, *defs, "-c", os.path.join(CSRC, src), "-o", objs[i]]
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
         r = subprocess.run(cmd, capture_output=True, text=True)
