@@ -56,6 +56,8 @@ BATCH_WORDS = 10000
 MAX_DIM = 512
 TXT_MATRIX = 0
 TXT_W2V = 1
+F32, F16, BF16 = 0, 1, 2
+EMBED_MAX_DIM = 1048576
 SUPPORTED_NEGATIVE = tuple(range(1, 21))
 
 
@@ -126,6 +128,15 @@ SIGNATURES = {
     "g2v_comm_abort": (C.c_int, [_vp]),
     "g2v_read_stats": (C.c_int, [_vp, C.POINTER(Stats)]),
     "g2v_cosine_pairs": (C.c_int, [C.c_int, _vp, _i64, _i32, _vp, _vp, _i64, _vp]),
+    "g2v_embed_lookup": (C.c_int, [C.c_int, _vp, C.c_int, _i64, _i64, _i64, _vp, C.c_int, _i64,
+                                   _f32, _vp, C.c_int, _vp]),
+    "g2v_embed_grad_workspace": (C.c_int, [_i64, _i64, _i64, C.POINTER(_i64)]),
+    "g2v_embed_grad": (C.c_int, [C.c_int, _vp, C.c_int, _i64, _vp, C.c_int, _i64, _i64, _i64, _f32,
+                                 _i64, _vp, C.c_int, _vp, _i64, _vp]),
+    "g2v_global_norm_workspace": (C.c_int, [_i64, C.POINTER(_i64)]),
+    "g2v_global_norm": (C.c_int, [C.c_int, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp]),
+    "g2v_clip_global_norm": (C.c_int, [C.c_int, _vp, _vp, _vp, _vp, _i64, _f64, _vp, _vp, _i64,
+                                       _vp]),
     "g2v_permute_items8": (C.c_int, [C.c_int, _vp, _vp, _i64, _i64, _i64, C.c_uint64, _vp]),
     "g2v_first_occurrence_perm8": (C.c_int, [C.c_int, _vp, _i64, C.c_uint64, _i32, _vp, _vp]),
     "g2v_seeded_vectors": (C.c_int, [_vp, _i64, _i32, _vp]),

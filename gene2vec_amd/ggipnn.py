@@ -9,12 +9,17 @@ pipeline, architecture, initialisers and optimiser:
          occurrence over lines with exactly 2 space-separated genes), ids via
          myFit (lines without 2 genes stay [1, 1]), one-hot labels
   embed  GGIPNN_util.load_embedding_vectors: U(-0.25, 0.25) then rows found in
-         the .txt (line.split()); frozen (train_embedding=False, GGIPNN.py:19-21)
+         the .txt (line.split()); frozen unless train_embedding=True
+         (GGIPNN.py:19-21).  On the GPU the lookup and the gradient of its
+         table are ``ops.embedding_lookup``, on the CPU torch indexing
   model  GGIPNN.py:25-69 -- concat(2 x D) -> 100 -> 100 -> 10 -> 2, ReLU,
          dropout keep 0.5 after each hidden layer, biases 0.1, weights
          variance_scaling (factor 2, fan_in, truncated normal)
   train  Adam(1e-3), batch 128, 1 epoch, softmax cross-entropy, l2 = 0
-         (GGIPNN_Classification.py:15-30,123-127,208-221)
+         (GGIPNN_Classification.py:15-30,123-127,208-221); clip_norm (not in
+         the reference): the gradients' global norm is held to it before each
+         step (tf.clip_by_global_norm's rule), on the GPU by
+         ``ops.clip_by_global_norm_``
   score  test AUC of softmax[:, 1] (sklearn roc_auc_score, :238-254)
 
 Randomness (unseeded in the reference) is driven by one ``seed`` here.
@@ -98,7 +103,26 @@ def _variance_scaling_(w, gen):
         w.copy_(t * std)
 
 
-def build_model(vocab_size, emb, embedding_size, device, gen):
+def clip_gradients_(params, clip_norm):
+    """scale the gradients in place by clip_norm / max(norm, clip_norm), norm
+    over all of them (NaN everywhere if it is not finite); returns the norm"""
+    import torch
+    if not 0.0 < clip_norm < math.inf:
+        raise ValueError(f"clip_norm must be positive and finite, not {clip_norm}")
+    grads = [p.grad for p in params if p.grad is not None]
+    if not grads:
+        raise ValueError("no parameter has a gradient")
+    if all(g.is_cuda for g in grads):
+        from . import ops
+        return ops.clip_by_global_norm_(grads, clip_norm)
+    norm = torch.sqrt(sum(g.double().square().sum() for g in grads))
+    factor = torch.where(norm.isfinite(), clip_norm / norm.clamp(min=clip_norm), math.nan)
+    for g in grads:
+        g.mul_(factor.to(g.dtype))
+    return norm.float()
+
+
+def build_model(vocab_size, emb, embedding_size, device, gen, train_embedding=False):
     import torch
     import torch.nn as nn
 
@@ -106,7 +130,7 @@ def build_model(vocab_size, emb, embedding_size, device, gen):
         def __init__(self):
             super().__init__()
             self.W = nn.Parameter(torch.as_tensor(emb, dtype=torch.float32, device=device),
-                                  requires_grad=False)
+                                  requires_grad=bool(train_embedding))
             dims = [2 * embedding_size, 100, 100, 10, 2]
             self.ws = nn.ParameterList()
             self.bs = nn.ParameterList()
@@ -117,7 +141,12 @@ def build_model(vocab_size, emb, embedding_size, device, gen):
                 self.bs.append(nn.Parameter(torch.full((b,), 0.1, device=device)))
 
         def forward(self, x, keep_prob):
-            h = self.W[x].reshape(x.shape[0], -1)
+            if self.W.is_cuda:
+                from . import ops
+                h = ops.embedding_lookup(self.W, x)
+            else:
+                h = self.W[x]
+            h = h.reshape(x.shape[0], -1)
             for i in range(3):
                 h = torch.relu(h @ self.ws[i] + self.bs[i])
                 if keep_prob < 1.0:
@@ -129,7 +158,8 @@ def build_model(vocab_size, emb, embedding_size, device, gen):
 
 
 def train_and_auc(embedding_file, data_dir, seed=0, device="cpu", embedding_size=200,
-                  batch_size=128, num_epochs=1, keep_prob=0.5, lr=1e-3):
+                  batch_size=128, num_epochs=1, keep_prob=0.5, lr=1e-3, train_embedding=False,
+                  clip_norm=None):
     import torch
     from sklearn import metrics
 
@@ -151,7 +181,7 @@ def train_and_auc(embedding_file, data_dir, seed=0, device="cpu", embedding_size
     emb = load_embedding_vectors(voca, embedding_file, embedding_size, rng)
     gen = torch.Generator(device=device)
     gen.manual_seed(seed)
-    model = build_model(len(voca), emb, embedding_size, device, gen)
+    model = build_model(len(voca), emb, embedding_size, device, gen, train_embedding)
     opt = torch.optim.Adam([p for p in model.parameters() if p.requires_grad], lr=lr,
                            betas=(0.9, 0.999), eps=1e-8)
     xt = torch.as_tensor(x_train, device=device)
@@ -165,6 +195,8 @@ def train_and_auc(embedding_file, data_dir, seed=0, device="cpu", embedding_size
             loss = torch.nn.functional.cross_entropy(logits, yt[idx])
             opt.zero_grad()
             loss.backward()
+            if clip_norm is not None:
+                clip_gradients_(model.parameters(), clip_norm)
             opt.step()
     with torch.no_grad():
         scores = torch.softmax(model(torch.as_tensor(x_test, device=device), 1.0), dim=1)[:, 1]

@@ -458,6 +458,58 @@ int g2v_coexpr_last_timing(double *mask_ms, double *total_ms);
 int g2v_cosine_pairs(int device, const float *vectors, int64_t V, int32_t D, const int32_t *a,
                      const int32_t *b, int64_t n, float *out);
 
+/* ---- tensor operators ---------------------------------------------------------------- */
+/* What a classifier over the embeddings (src/GGIPNN.py) trains with: the lookup
+ * of its table, the gradient of that table, the global norm of its gradients
+ * and clipping.  All pointers are device memory of `device` (the lists of
+ * pointers, sizes and types are host memory, read during the call); work is
+ * enqueued on `stream` (a hipStream_t of that device, NULL: the null stream)
+ * without synchronisation, allocation or host copies, so the calls may be
+ * captured into a HIP graph.  The caller's current device is left as it was.
+ * Workspaces are the caller's: 16-byte aligned, of at least the size asked
+ * for, holding nothing between calls; calls that may run at the same time
+ * need one each.  Pointers are aligned to their element type, no more.  The
+ * same inputs give the same bits. */
+#define G2V_F32 0
+#define G2V_F16 1
+#define G2V_BF16 2
+#define G2V_EMBED_MAX_DIM 1048576
+
+/* out[i][d] = scale * table[ids[i]][d] for i < n, d < D, formed in fp32 and
+ * rounded once; a zero row where ids[i] is outside [0, V).  table: V rows of
+ * D elements every ld elements; out: dense [n][D]; ids: int32 (id_bytes 4) or
+ * int64 (8).  tf.nn.embedding_lookup (src/GGIPNN.py:24), absent tokens added. */
+int g2v_embed_lookup(int device, const void *table, int table_type, int64_t V, int64_t D,
+                     int64_t ld, const void *ids, int id_bytes, int64_t n, float scale, void *out,
+                     int out_type, void *stream);
+
+/* grad[v][d] = scale * (sum over i with ids[i] == v of dy[i][d]) for every v < V:
+ * dense [V][D], every row written (zeros where no id names it, and for
+ * padding_id; -1: none).  ids outside [0, V) add nothing.  dy: n rows of D
+ * elements every dy_ld elements.  Sums are fp32 in a fixed order, without
+ * atomics; one rounding to grad_type. */
+int g2v_embed_grad_workspace(int64_t n, int64_t V, int64_t D, int64_t *bytes);
+int g2v_embed_grad(int device, const void *dy, int dy_type, int64_t dy_ld, const void *ids,
+                   int id_bytes, int64_t n, int64_t V, int64_t D, float scale, int64_t padding_id,
+                   void *grad, int grad_type, void *workspace, int64_t workspace_bytes,
+                   void *stream);
+
+/* *norm = sqrt(sum of the squares of all elements of the n tensors), squares
+ * and sums in fp64 (tf.global_norm).  tensors[t]: numel[t] contiguous elements
+ * of types[t]; empty tensors may be NULL. */
+int g2v_global_norm_workspace(int64_t n, int64_t *bytes);
+int g2v_global_norm(int device, const void *const *tensors, const int64_t *numel,
+                    const int32_t *types, int64_t n, float *norm, void *workspace,
+                    int64_t workspace_bytes, void *stream);
+
+/* dst[t] = src[t] * (clip_norm / max(norm, clip_norm)), the factor rounded to
+ * fp32 and the product once to the type; *norm as above, before clipping
+ * (tf.clip_by_global_norm).  A norm that is not finite makes every element
+ * NaN.  dst[t] == src[t] clips in place; any other overlap is refused. */
+int g2v_clip_global_norm(int device, const void *const *src, void *const *dst,
+                         const int64_t *numel, const int32_t *types, int64_t n, double clip_norm,
+                         float *norm, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* ---- device reshuffle of a pair corpus ------------------------------------------- */
 /* The per-iteration reshuffle of src/gene2vec.py:80 (random.shuffle, unseeded
  * there) for a corpus resident in HBM: dst[i] = src[p(first + i)] for i < count,

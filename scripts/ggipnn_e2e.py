@@ -112,9 +112,10 @@ def cosine_auc(emb):
     return float(metrics.roc_auc_score(lab, s))
 
 
-def auc(emb, seeds):
+def auc(emb, seeds, device="cpu", train_embedding=False, clip_norm=None):
     from gene2vec_amd import ggipnn as G
-    vals = [G.train_and_auc(emb, DATA, seed=s) for s in seeds]
+    vals = [G.train_and_auc(emb, DATA, seed=s, device=device, train_embedding=train_embedding,
+                            clip_norm=clip_norm) for s in seeds]
     out = {"emb": emb, "seeds": seeds, "auc": vals, "mean": float(np.mean(vals)),
            "std": float(np.std(vals)), "cosine_auc": cosine_auc(emb)}
     print(json.dumps(out))
@@ -130,8 +131,13 @@ if __name__ == "__main__":
     p.add_argument("--seed", type=int, default=7)
     p.add_argument("--emb")
     p.add_argument("--seeds", default="0,1,2,3,4")
+    p.add_argument("--device", default="cpu", help="auc: where the classifier trains")
+    p.add_argument("--train-embedding", action="store_true",
+                   help="auc: the classifier trains its embedding table too")
+    p.add_argument("--clip-norm", type=float,
+                   help="auc: hold the gradients' global norm to this before each step")
     a = p.parse_args()
     if a.cmd == "train":
         train(a.engine, a.out, a.iters, a.seed)
     else:
-        auc(a.emb, [int(s) for s in a.seeds.split(",")])
+        auc(a.emb, [int(s) for s in a.seeds.split(",")], a.device, a.train_embedding, a.clip_norm)
