@@ -16,15 +16,55 @@ using g2v::f16;
 
 constexpr int kThreads = 256;
 
-template <class TW, class TY, class I>
+constexpr int kUnits = 4;  // vectors a thread of the lookup moves
+
+// The elements of a vector: 16 bytes of the narrower of the two types.  A row
+// of D elements is ceil(D / VEC) vectors; the last one ends with the row and
+// overlaps the one before where VEC does not divide D (the same values are
+// written twice), so that no width needs a scalar tail.  Rows narrower than a
+// vector go element by element.
+template <class A, class B>
+constexpr int vec_of() {
+  return 16 / (sizeof(A) < sizeof(B) ? sizeof(A) : sizeof(B));
+}
+
+// Memory bound: a row read and a row written per token, no reuse.  Vectors of
+// all rows are numbered through and dealt out 1024 to a workgroup, so every
+// width fills the lanes and one row is spread over as many threads as it has
+// vectors; kUnits independent id -> row chains per thread cover the latency.
+template <class TW, class TY, class I, int VEC>
 __global__ __launch_bounds__(kThreads) void k_embed_lookup(
-    const TW* __restrict__ W, int64_t V, int64_t D, int64_t ld, const I* __restrict__ ids,
-    int64_t n, float scale, TY* __restrict__ out) {
-  const int64_t step = (int64_t)gridDim.x * kThreads;
-  for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < n * D; e += step) {
-    const int64_t i = e / D, id = ids[i];
-    out[e] = (TY)(id >= 0 && id < V ? (float)W[id * ld + (e - i * D)] * scale : 0.f);
+    const TW* __restrict__ W, int64_t V, int D, int64_t ld, const I* __restrict__ ids,
+    int64_t units, int nv, float scale, TY* __restrict__ out) {
+  const int64_t u0 = (int64_t)blockIdx.x * (kThreads * kUnits);
+  const int64_t row0 = u0 / nv;
+  const uint32_t r0 = (uint32_t)(u0 - row0 * nv) + threadIdx.x;  // < nv + 1024
+  const int64_t left = units - u0;
+  int64_t id[kUnits], at[kUnits];
+  int col[kUnits];
+  float x[kUnits][VEC];
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k) {
+    const uint32_t l = r0 + k * kThreads, q = l / (uint32_t)nv;
+    const int c = (int)(l - q * nv) * VEC;
+    col[k] = c + VEC <= D ? c : D - VEC;
+    at[k] = row0 + q;
+    id[k] = (int)threadIdx.x + k * kThreads < left ? (int64_t)ids[at[k]] : -1;
   }
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[k][i] = 0.f;
+    if (id[k] >= 0 && id[k] < V) {
+      g2v::load_vec<TW, VEC>(W + id[k] * ld + col[k], x[k]);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) x[k][i] *= scale;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k)
+    if ((int)threadIdx.x + k * kThreads < left)
+      g2v::store_vec<TY, VEC>(out + at[k] * D + col[k], x[k]);
 }
 
 // one wave per row and 64 columns: the ids in order, 64 at a time, and the
@@ -113,19 +153,28 @@ extern "C" int g2v_embed_lookup(int device, const void* table, int table_type, i
   g2v::DeviceScope scope(device);
   OP_HIP(scope.error(), what);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  by_type(table_type, [&](auto w) {
+  rc = by_type(table_type, [&](auto w) {
     return by_type(out_type, [&](auto y) {
       return by_id(id_bytes, [&](auto i) {
         using TW = decltype(w);
         using TY = decltype(y);
         using I = decltype(i);
-        hipLaunchKernelGGL((k_embed_lookup<TW, TY, I>), dim3(grid_for(n * D, kThreads)),
-                           dim3(kThreads), 0, st, static_cast<const TW*>(table), V, D, ld,
-                           static_cast<const I*>(ids), n, scale, static_cast<TY*>(out));
-        return 0;
+        constexpr int VEC = vec_of<TW, TY>();
+        const int64_t nv = D >= VEC ? (D + VEC - 1) / VEC : D;
+        const int64_t blocks = (n * nv + kThreads * kUnits - 1) / (kThreads * kUnits);
+        // a launch is limited to 2^32 threads
+        OP_REQUIRE(blocks < (int64_t)1 << 24, G2V_ERANGE, "%s: %lld x %lld elements in one call",
+                   what, (long long)n, (long long)D);
+        hipLaunchKernelGGL((D >= VEC ? k_embed_lookup<TW, TY, I, VEC> : k_embed_lookup<TW, TY, I, 1>),
+                           dim3((unsigned)blocks), dim3(kThreads), 0, st,
+                           static_cast<const TW*>(table), V, (int)D, ld,
+                           static_cast<const I*>(ids), n * nv, (int)nv, scale,
+                           static_cast<TY*>(out));
+        return (int)G2V_OK;
       });
     });
   });
+  if (rc != G2V_OK) return rc;
   OP_HIP(hipGetLastError(), what);
   return G2V_OK;
 }

@@ -80,21 +80,52 @@ __device__ __forceinline__ void my_chunks(const Tensors& a, int& c0, int& c1) {
   c1 = (int)(chunks * (blockIdx.x + 1) / gridDim.x);
 }
 
+// x[0 .. n) of p by the workgroup's threads, 16 bytes an access; f(first
+// element, values, their number).  A full chunk is unrolled: all its loads are
+// in flight at once.  The tail goes element by element.
+template <class T, class F>
+__device__ __forceinline__ void for_vectors(const T* p, int n, F f) {
+  constexpr int VEC = 16 / sizeof(T), kStep = kThreads * VEC;
+  if (n == kChunk) {
+    float x[kChunk / kStep][VEC];
+#pragma unroll
+    for (int k = 0; k < kChunk / kStep; ++k)
+      g2v::load_vec<T, VEC>(p + k * kStep + threadIdx.x * VEC, x[k]);
+#pragma unroll
+    for (int k = 0; k < kChunk / kStep; ++k) f(k * kStep + threadIdx.x * VEC, x[k]);
+    return;
+  }
+  int i = threadIdx.x * VEC;
+  for (; i + VEC <= n; i += kStep) {
+    float x[VEC];
+    g2v::load_vec<T, VEC>(p + i, x);
+    f(i, x);
+  }
+  for (int e = i; e < n && e < i + VEC; ++e) {
+    float x[1] = {(float)p[e]};
+    f(e, x);
+  }
+}
+
 __global__ __launch_bounds__(kThreads) void k_square_sum(Tensors a, double* __restrict__ partial) {
   int c0, c1;
   my_chunks(a, c0, c1);
-  double s = 0.0;
+  double s0 = 0.0, s1 = 0.0;
   for_chunks(a, c0, c1, [&](int t, int64_t e, int n) {
     by_type_dev(a.type[t], [&](auto z) {
       using T = decltype(z);
-      const T* p = static_cast<const T*>(a.src[t]) + e;
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const double x = (double)(float)p[i];
-        s = fma(x, x, s);
-      }
+      for_vectors(static_cast<const T*>(a.src[t]) + e, n, [&](int, auto& x) {
+        constexpr int N = sizeof x / sizeof x[0];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const double d = (double)x[i];
+          if (i & 1) s1 = fma(d, d, s1);
+          else s0 = fma(d, d, s0);
+        }
+      });
     });
   });
-  s = block_sum(s);
+  const double s = block_sum(s0 + s1);
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
@@ -123,9 +154,13 @@ __global__ __launch_bounds__(kThreads) void k_clip(Tensors a, const double* __re
     if (f == 1.f && a.src[t] == a.dst[t]) return;  // in place and within the bound
     by_type_dev(a.type[t], [&](auto z) {
       using T = decltype(z);
-      const T* p = static_cast<const T*>(a.src[t]) + e;
       T* q = static_cast<T*>(a.dst[t]) + e;
-      for (int i = threadIdx.x; i < n; i += kThreads) q[i] = (T)((float)p[i] * f);
+      for_vectors(static_cast<const T*>(a.src[t]) + e, n, [&](int at, auto& x) {
+        constexpr int N = sizeof x / sizeof x[0];
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] *= f;
+        g2v::store_vec<T, N>(q + at, x);
+      });
     });
   });
 }
