@@ -16,6 +16,15 @@ using g2v::f16;
 
 constexpr int kThreads = 256;
 
+// workgroups are numbered over two grid dimensions: one holds 2^32 threads
+inline dim3 grid_of(int64_t blocks) {
+  const int64_t x = blocks < 1 << 20 ? blocks : 1 << 20;
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+__device__ __forceinline__ int64_t block_number() {
+  return (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+}
+
 constexpr int kUnits = 4;  // vectors a thread of the lookup moves
 
 // The elements of a vector: 16 bytes of the narrower of the two types.  A row
@@ -36,7 +45,7 @@ template <class TW, class TY, class I, int VEC>
 __global__ __launch_bounds__(kThreads) void k_embed_lookup(
     const TW* __restrict__ W, int64_t V, int D, int64_t ld, const I* __restrict__ ids,
     int64_t units, int nv, float scale, TY* __restrict__ out) {
-  const int64_t u0 = (int64_t)blockIdx.x * (kThreads * kUnits);
+  const int64_t u0 = block_number() * (kThreads * kUnits);
   const int64_t row0 = u0 / nv;
   const uint32_t r0 = (uint32_t)(u0 - row0 * nv) + threadIdx.x;  // < nv + 1024
   const int64_t left = units - u0;
@@ -67,31 +76,451 @@ __global__ __launch_bounds__(kThreads) void k_embed_lookup(
       g2v::store_vec<TY, VEC>(out + at[k] * D + col[k], x[k]);
 }
 
-// one wave per row and 64 columns: the ids in order, 64 at a time, and the
-// rows of dy whose id is this one
-template <class TY, class TG, class I>
-__global__ __launch_bounds__(kThreads) void k_embed_grad_direct(
-    const TY* __restrict__ dy, int64_t dy_ld, const I* __restrict__ ids, int64_t n, int64_t V,
-    int64_t D, float scale, int64_t pad, TG* __restrict__ grad) {
+// ---- the gradient: tokens sorted by row, then one sum per row --------------------
+//
+// The sort is stable (tokens of a row stay in token order) and uses no atomics
+// on memory, so the order of every sum, and with it the result, is fixed.
+// Rows are dealt to kBuckets buckets by their low bits: frequent rows, mostly
+// neighbours in a vocabulary sorted by count, fall into different buckets.
+// Inside a bucket a workgroup counts its rows in LDS, wave by wave over
+// consecutive slices of the tokens, scans the counts and places the tokens.
+//
+// Up to kScanTokens tokens every bucket's workgroup reads all ids itself: it
+// picks its own and counts those of lower buckets, which is where its part of
+// the sorted list begins.  One launch, no exchange between workgroups.  Beyond
+// that the tokens are split into buckets first (tile histograms, then a stable
+// scatter), and every workgroup reads its bucket alone.
+
+constexpr int kBuckets = 256;
+constexpr int kSortThreads = 1024;
+constexpr int kSortWaves = kSortThreads / 64;
+constexpr int kKeys = 768;       // rows a bucket counts at a time (48 KB of LDS)
+constexpr int kTileTokens = 8192;
+constexpr int kMaxTiles = 256;   // larger calls take larger tiles
+constexpr int64_t kScanTokens = 65536;
+constexpr int kJoinSplit = 4;    // workgroups per bucket that join long runs
+
+struct Sorted {
+  int32_t* perm;    // [n] token positions, row by row
+  int32_t* start;   // [V] first place of row v in perm
+  int32_t* count;   // [V]
+  int32_t* at;      // [n / L + 1] row at every L-th place of perm
+  int32_t* longs;   // [n / L + 1] rows of more than L tokens, bucket by bucket
+  int32_t* nlong;   // [kBuckets] how many of them
+  int32_t* lfirst;  // [kBuckets] where the bucket's begin
+  int32_t* total;   // tokens that name a row
+  int log2L;
+};
+
+// the lanes of the wave whose key equals this lane's, among those that have one
+__device__ __forceinline__ uint64_t peers(int key, bool has, int bits) {
+  uint64_t m = __ballot(has);
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (key >> b) & 1;
+    const uint64_t o = __ballot(one);
+    m &= one ? o : ~o;
+  }
+  return m;
+}
+
+// f(i, key(i)) for the tokens [i0, i1) in order, 64 at a time by a whole wave,
+// -1 past the end; four loads in flight
+template <class K, class F>
+__device__ __forceinline__ void for_slice(int64_t i0, int64_t i1, K key, F f) {
   const int lane = threadIdx.x & 63;
-  const int64_t tiles = (D + 63) / 64, items = V * tiles;
-  const int64_t step = (int64_t)gridDim.x * (kThreads / 64);
-  for (int64_t it = (int64_t)blockIdx.x * (kThreads / 64) + threadIdx.x / 64; it < items;
-       it += step) {
-    const int64_t v = it / tiles, col = (it - v * tiles) * 64 + lane;
-    float acc = 0.f;
-    if (v != pad) {
-      for (int64_t b = 0; b < n; b += 64) {
-        uint64_t m = __ballot(b + lane < n && (int64_t)ids[b + lane < n ? b + lane : 0] == v);
-        while (m) {
-          const int64_t i = b + __builtin_ctzll(m);
-          m &= m - 1;
-          if (col < D) acc += (float)dy[i * dy_ld + col];
-        }
+  for (int64_t i = i0; i < i1; i += 256) {
+    int k[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t j = i + u * 64 + lane;
+      k[u] = j < i1 ? key(j) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) f(i + u * 64 + lane, k[u]);
+  }
+}
+
+// the slice of n tokens that this wave takes: whole groups of 64, in wave order
+__device__ __forceinline__ void my_slice(int64_t n, int64_t& i0, int64_t& i1) {
+  const int64_t per = (n + kSortThreads - 1) / kSortThreads * 64;
+  i0 = (int64_t)(threadIdx.x / 64) * per;
+  i0 = i0 < n ? i0 : n;
+  i1 = i0 + per < n ? i0 + per : n;
+}
+
+// exclusive sum over the workgroup, and the sum in all
+__device__ __forceinline__ int block_scan(int x, int& all) {
+  __shared__ int wsum[kSortWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+  int s = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int t = __shfl_up(s, d);
+    if (lane >= d) s += t;
+  }
+  if (lane == 63) wsum[wave] = s;
+  __syncthreads();
+  int before = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kSortWaves; ++w) {
+    if (w < wave) before += wsum[w];
+    all += wsum[w];
+  }
+  __syncthreads();
+  return before + s - x;
+}
+
+// count[key] += the wave's tokens of that key
+__device__ __forceinline__ void count_keys(uint32_t* count, int key, bool has, int bits) {
+  if (!__ballot(has)) return;
+  const uint64_t m = peers(key, has, bits);
+  if (has && __builtin_ctzll(m) == (int)(threadIdx.x & 63)) atomicAdd(&count[key], __popcll(m));
+}
+
+// the place of this lane's token: next[key] plus the lower lanes of that key;
+// next[key] moves on by all of them
+__device__ __forceinline__ int place_keys(uint32_t* next, int key, bool has, int bits) {
+  const int lane = threadIdx.x & 63;
+  const uint64_t m = peers(key, has, bits);
+  const int lead = has ? __builtin_ctzll(m) : lane;
+  int old = 0;
+  if (has && lead == lane) old = (int)atomicAdd(&next[key], __popcll(m));
+  return __shfl(old, lead) + __popcll(m & ((1ull << lane) - 1));
+}
+
+// Sorts the tokens of bucket b.  key(i, below): the row of token i over
+// kBuckets, -1 if it is none of b's, below counting the tokens of lower
+// buckets; pos(i): its position.  base: where the bucket begins, less those.
+template <class K, class P>
+__device__ __forceinline__ void sort_bucket(int b, int V, int64_t n, int base, const Sorted& s,
+                                            K key, P pos) {
+  __shared__ uint32_t hist[kSortWaves * kKeys];
+  __shared__ int nlong;
+  const int rows = V > b ? (V - b + kBuckets - 1) / kBuckets : 0;
+  uint32_t* mine = hist + (threadIdx.x / 64) * kKeys;
+  int64_t i0, i1;
+  my_slice(n, i0, i1);
+  int first = 0;
+  if (threadIdx.x == 0) nlong = 0;
+  for (int w0 = 0; w0 == 0 || w0 < rows; w0 += kKeys) {
+    const int rw = rows - w0 < kKeys ? rows - w0 : kKeys;
+    const int bits = rw > 1 ? 32 - __builtin_clz(rw - 1) : 0;
+    for (int k = threadIdx.x; k < kSortWaves * kKeys; k += kSortThreads) hist[k] = 0;
+    __syncthreads();
+    int below = 0;
+    for_slice(i0, i1, [&](int64_t i) { return key(i, below); },
+              [&](int64_t, int k) {
+                k -= w0;
+                count_keys(mine, k, k >= 0 && k < rw, bits);
+              });
+    __syncthreads();
+    if (w0 == 0) {
+      int all;
+      (void)block_scan(below, all);
+      base += all;
+      first = base >> s.log2L;
+    }
+    const int t = threadIdx.x;
+    int c = 0, all;
+    if (t < rw)
+      for (int w = 0; w < kSortWaves; ++w) c += (int)hist[w * kKeys + t];
+    int at = base + block_scan(c, all);
+    if (t < rw) {
+      const int v = (w0 + t) * kBuckets + b;
+      s.start[v] = at;
+      s.count[v] = c;
+      if (c > 1 << s.log2L) s.longs[first + atomicAdd(&nlong, 1)] = v;
+      for (int w = 0; w < kSortWaves; ++w) {
+        const int h = (int)hist[w * kKeys + t];
+        hist[w * kKeys + t] = (uint32_t)at;
+        at += h;
       }
     }
-    if (col < D) grad[v * D + col] = (TG)(acc * scale);
+    __syncthreads();
+    for_slice(i0, i1, [&](int64_t i) { int none = 0; return key(i, none); },
+              [&](int64_t i, int k) {
+                const int kw = k - w0;
+                const bool has = kw >= 0 && kw < rw;
+                if (!__ballot(has)) return;
+                const int p = place_keys(mine, kw, has, bits);
+                if (!has) return;
+                s.perm[p] = pos(i);
+                if ((p & ((1 << s.log2L) - 1)) == 0) s.at[p >> s.log2L] = k * kBuckets + b;
+              });
+    base += all;
+    __syncthreads();
   }
+  if (threadIdx.x == 0) {
+    s.nlong[b] = nlong;
+    s.lfirst[b] = first;
+    if (b == kBuckets - 1) *s.total = base;
+  }
+}
+
+// the row of a token, -1 if it names none or the padding
+template <class I>
+__device__ __forceinline__ int row_of(const I* __restrict__ ids, int64_t i, int V, int pad) {
+  const int64_t id = (int64_t)ids[i];
+  return id >= 0 && id < V && id != pad ? (int)id : -1;
+}
+
+template <class I>
+__global__ __launch_bounds__(kSortThreads) void k_sort_scan(const I* __restrict__ ids, int64_t n,
+                                                            int V, int pad, Sorted s) {
+  const int b = blockIdx.x;
+  sort_bucket(b, V, n, 0, s,
+              [&](int64_t i, int& below) {
+                const int v = row_of(ids, i, V, pad), d = v & (kBuckets - 1);
+                below += v >= 0 && d < b;
+                return v >= 0 && d == b ? v / kBuckets : -1;
+              },
+              [](int64_t i) { return (int)i; });
+}
+
+// tokens of every bucket in every tile
+template <class I>
+__global__ __launch_bounds__(kSortThreads) void k_tile_count(const I* __restrict__ ids, int64_t n,
+                                                             int64_t tile, int V, int pad,
+                                                             int32_t* __restrict__ counts) {
+  __shared__ uint32_t hist[kSortWaves * kBuckets];
+  const int64_t t0 = (int64_t)blockIdx.x * tile, len = n - t0 < tile ? n - t0 : tile;
+  for (int k = threadIdx.x; k < kSortWaves * kBuckets; k += kSortThreads) hist[k] = 0;
+  __syncthreads();
+  int64_t i0, i1;
+  my_slice(len, i0, i1);
+  uint32_t* mine = hist + (threadIdx.x / 64) * kBuckets;
+  for_slice(i0, i1, [&](int64_t i) { return row_of(ids, t0 + i, V, pad); },
+            [&](int64_t, int v) { count_keys(mine, v & (kBuckets - 1), v >= 0, 8); });
+  __syncthreads();
+  if (threadIdx.x < kBuckets) {
+    uint32_t c = 0;
+    for (int w = 0; w < kSortWaves; ++w) c += hist[w * kBuckets + threadIdx.x];
+    counts[blockIdx.x * kBuckets + threadIdx.x] = (int32_t)c;
+  }
+}
+
+// the tokens as (row, position), bucket by bucket, in token order within one
+template <class I>
+__global__ __launch_bounds__(kSortThreads) void k_tile_scatter(
+    const I* __restrict__ ids, int64_t n, int64_t tile, int V, int pad,
+    const int32_t* __restrict__ counts, int32_t* __restrict__ bfirst, int2* __restrict__ pairs) {
+  __shared__ uint32_t hist[kSortWaves * kBuckets];
+  __shared__ int tsum[2][kSortThreads / kBuckets][kBuckets];
+  const int64_t t0 = (int64_t)blockIdx.x * tile, len = n - t0 < tile ? n - t0 : tile;
+  for (int k = threadIdx.x; k < kSortWaves * kBuckets; k += kSortThreads) hist[k] = 0;
+  const int d = threadIdx.x % kBuckets, g = threadIdx.x / kBuckets;
+  int before = 0, every = 0;
+  for (int t = g; t < (int)gridDim.x; t += kSortThreads / kBuckets) {
+    const int c = counts[t * kBuckets + d];
+    every += c;
+    before += t < (int)blockIdx.x ? c : 0;
+  }
+  tsum[0][g][d] = before;
+  tsum[1][g][d] = every;
+  __syncthreads();
+  int64_t i0, i1;
+  my_slice(len, i0, i1);
+  uint32_t* mine = hist + (threadIdx.x / 64) * kBuckets;
+  for_slice(i0, i1, [&](int64_t i) { return row_of(ids, t0 + i, V, pad); },
+            [&](int64_t, int v) { count_keys(mine, v & (kBuckets - 1), v >= 0, 8); });
+  before = every = 0;
+  if (threadIdx.x < kBuckets)
+    for (int q = 0; q < kSortThreads / kBuckets; ++q) {
+      before += tsum[0][q][d];
+      every += tsum[1][q][d];
+    }
+  int all;
+  const int b0 = block_scan(every, all);  // the bucket's first place (a barrier inside)
+  if (threadIdx.x < kBuckets) {
+    if (blockIdx.x == 0) {
+      bfirst[d] = b0;
+      if (d == 0) bfirst[kBuckets] = all;
+    }
+    uint32_t at = (uint32_t)(b0 + before);
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t h = hist[w * kBuckets + d];
+      hist[w * kBuckets + d] = at;
+      at += h;
+    }
+  }
+  __syncthreads();
+  for_slice(i0, i1, [&](int64_t i) { return row_of(ids, t0 + i, V, pad); },
+            [&](int64_t i, int v) {
+              if (!__ballot(v >= 0)) return;
+              const int p = place_keys(mine, v & (kBuckets - 1), v >= 0, 8);
+              if (v >= 0) pairs[p] = make_int2(v, (int)(t0 + i));
+            });
+}
+
+__global__ __launch_bounds__(kSortThreads) void k_sort_bucket(const int2* __restrict__ pairs,
+                                                              const int32_t* __restrict__ bfirst,
+                                                              int V, Sorted s) {
+  const int b = blockIdx.x, lo = bfirst[b];
+  sort_bucket(b, V, bfirst[b + 1] - lo, lo, s,
+              [&](int64_t i, int&) { return pairs[lo + i].x / kBuckets; },
+              [&](int64_t i) { return pairs[lo + i].y; });
+}
+
+// acc += the rows perm[p0 .. p1) of dy, in that order, eight loads in flight
+template <class TY, int VEC>
+__device__ __forceinline__ void sum_rows(const TY* __restrict__ dy, int64_t ld,
+                                         const int32_t* __restrict__ perm, int p0, int p1,
+                                         float (&acc)[VEC]) {
+  auto some = [&](auto many) {
+    constexpr int M = decltype(many)::value;
+    int64_t r[M];
+    float x[M][VEC];
+#pragma unroll
+    for (int m = 0; m < M; ++m) r[m] = perm[p0 + m];
+#pragma unroll
+    for (int m = 0; m < M; ++m) g2v::load_vec<TY, VEC>(dy + r[m] * ld, x[m]);
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] += x[m][i];
+    p0 += M;
+  };
+  while (p1 - p0 >= 8) some(std::integral_constant<int, 8>{});
+  if ((p1 - p0) & 4) some(std::integral_constant<int, 4>{});
+  if ((p1 - p0) & 2) some(std::integral_constant<int, 2>{});
+  if ((p1 - p0) & 1) some(std::integral_constant<int, 1>{});
+}
+
+// G lanes per row and G vectors of columns: the sum of a row of at most L
+// tokens goes to grad, of none zeros.  A longer run is cut at every L-th of its
+// tokens into pieces for groups of their own, first in the grid as they take
+// longest; their sums go to part.  Pieces are found by place: a run of more
+// than L tokens that begins in [cL, cL + L) covers the place (c + 1) L, and one
+// that begins before cL and has a piece there covers cL.  So slot 2c is the
+// first piece of the run that begins there, slot 2c + 1 a later piece of one
+// that began before; each exists at most once, as two such runs begin more
+// than L places apart.
+template <class TY, class TG, int VEC, int G>
+__global__ __launch_bounds__(kThreads) void k_grad_rows(const TY* __restrict__ dy, int64_t ld,
+                                                        Sorted s, float* __restrict__ part,
+                                                        int64_t V, int D, int nv, int tiles,
+                                                        int64_t slots, float scale,
+                                                        TG* __restrict__ grad) {
+  const int64_t it = block_number() * (kThreads / G) + threadIdx.x / G;
+  const int64_t row = tiles == 1 ? it : it / tiles;
+  const int unit = (int)(it - row * tiles) * G + threadIdx.x % G;
+  if (unit >= nv) return;
+  const int col = unit * VEC + VEC <= D ? unit * VEC : D - VEC;
+  float acc[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+  const int L = 1 << s.log2L;
+  if (row < slots) {
+    const int c = (int)(row >> 1), later = (int)(row & 1);
+    const int64_t q = (int64_t)(c + 1 - later) << s.log2L;
+    if (q >= *s.total) return;
+    const int v = s.at[c + 1 - later], p = s.start[v], n = s.count[v];
+    if (n <= L) return;
+    int p0 = p;
+    if (later) {
+      if (p >= q) return;
+      const int64_t e = p + ((q - p + L - 1) >> s.log2L << s.log2L);
+      if (e >= (int64_t)p + n) return;
+      p0 = (int)e;
+    } else if (p >> s.log2L != c) {
+      return;
+    }
+    sum_rows<TY, VEC>(dy + col, ld, s.perm, p0, p + n - p0 > L ? p0 + L : p + n, acc);
+    g2v::store_vec<float, VEC>(part + row * D + col, acc);
+    return;
+  }
+  const int64_t v = row - slots;
+  if (v >= V) return;
+  const int n = s.count[v];
+  if (n > L) return;
+  if (n > 0) {
+    const int p = s.start[v];
+    sum_rows<TY, VEC>(dy + col, ld, s.perm, p, p + n, acc);
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) acc[i] *= scale;
+  g2v::store_vec<TG, VEC>(grad + v * D + col, acc);
+}
+
+// a long run's pieces, added in order by kSortWaves waves in turn and those by
+// the first: a workgroup per bucket, share of its long runs, and 64 vectors
+template <class TG, int VEC>
+__global__ __launch_bounds__(kSortThreads) void k_grad_join(Sorted s,
+                                                            const float* __restrict__ part, int D,
+                                                            int nv, float scale,
+                                                            TG* __restrict__ grad) {
+  __shared__ float sums[kSortWaves][64][VEC];
+  const int b = blockIdx.x % kBuckets, lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+  const int nlong = s.nlong[b], first = s.lfirst[b];
+  const int unit = (int)blockIdx.y * 64 + lane;
+  const bool in = unit < nv;
+  const int col = !in ? 0 : unit * VEC + VEC <= D ? unit * VEC : D - VEC;
+  for (int j = blockIdx.x / kBuckets; j < nlong; j += kJoinSplit) {
+    const int v = s.longs[first + j], n = s.count[v];
+    const int pieces = (n + (1 << s.log2L) - 1) >> s.log2L;
+    const int64_t c0 = s.start[v] >> s.log2L;
+    float acc[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+    if (in) {
+#pragma unroll 4
+      for (int k = wave; k < pieces; k += kSortWaves) {
+        float x[VEC];
+        g2v::load_vec<float, VEC>(part + (2 * (c0 + k) + (k > 0)) * D + col, x);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] += x[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sums[wave][lane][i] = acc[i];
+    __syncthreads();
+    if (wave == 0 && in) {
+      for (int w = 1; w < kSortWaves; ++w)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] += sums[w][lane][i];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] *= scale;
+      g2v::store_vec<TG, VEC>(grad + (int64_t)v * D + col, acc);
+    }
+    __syncthreads();
+  }
+}
+
+// where everything lies in the workspace
+struct Plan {
+  int log2L;
+  int64_t chunks, slots;  // places of L tokens; pieces (none where no run can be long)
+  int64_t tiles, tile;    // 0: every bucket reads all ids
+  int64_t perm, start, count, at, longs, small, part, pairs, counts, bfirst, bytes;
+};
+
+Plan plan(int64_t n, int64_t V, int64_t D) {
+  Plan p{};
+  p.log2L = n <= 65536 ? 6 : n <= 262144 ? 7 : 8;
+  p.chunks = (n + ((int64_t)1 << p.log2L) - 1) >> p.log2L;
+  p.slots = n > (int64_t)1 << p.log2L ? 2 * p.chunks : 0;
+  if (n > kScanTokens) {
+    p.tile = (n + kMaxTiles - 1) / kMaxTiles;
+    p.tile = p.tile < kTileTokens ? kTileTokens : (p.tile + kSortThreads - 1) / kSortThreads * kSortThreads;
+    p.tiles = (n + p.tile - 1) / p.tile;
+  }
+  const auto take = [&](int64_t count, int64_t size) {
+    const int64_t o = p.bytes;
+    p.bytes += (count * size + 255) / 256 * 256;
+    return o;
+  };
+  p.perm = take(n, 4);
+  p.start = take(V, 4);
+  p.count = take(V, 4);
+  p.at = take(p.chunks + 1, 4);
+  p.longs = take(p.chunks + 1, 4);
+  p.small = take(2 * kBuckets + 1, 4);
+  p.part = take(p.slots, 4 * D);
+  p.pairs = take(p.tiles ? n : 0, 8);
+  p.counts = take(p.tiles * kBuckets, 4);
+  p.bfirst = take(p.tiles ? kBuckets + 1 : 0, 4);
+  return p;
 }
 
 template <class F>
@@ -135,9 +564,60 @@ int check_matrix(const char* what, const char* name, const void* p, int type, in
   return G2V_OK;
 }
 
-unsigned grid_for(int64_t items, int64_t per_block) {
-  const int64_t g = (items + per_block - 1) / per_block;
-  return (unsigned)(g < 1 ? 1 : g > 8192 ? 8192 : g);
+template <class TY, class TG, int VEC>
+int launch_rows(const TY* dy, int64_t ld, const Sorted& s, const Plan& p, float* part, int64_t V,
+                int64_t D, float scale, TG* grad, hipStream_t st) {
+  const int64_t nv = D >= VEC ? (D + VEC - 1) / VEC : D;
+  const auto go = [&](auto kernel, int G) {
+    const int64_t tiles = (nv + G - 1) / G;
+    const int64_t blocks = ((p.slots + V) * tiles + kThreads / G - 1) / (kThreads / G);
+    hipLaunchKernelGGL(kernel, grid_of(blocks), dim3(kThreads), 0, st, dy, ld, s, part, V,
+                       (int)D, (int)nv, (int)tiles, p.slots, scale, grad);
+    OP_HIP(hipGetLastError(), "g2v_embed_grad");
+    return (int)G2V_OK;
+  };
+  // as few idle lanes as a power of two allows: a row of nv vectors on 64
+  // lanes would leave all but nv of them without work
+  if (D < VEC) return go(k_grad_rows<TY, TG, 1, 8>, 8);
+  if (nv <= 8) return go(k_grad_rows<TY, TG, VEC, 8>, 8);
+  if (nv <= 16) return go(k_grad_rows<TY, TG, VEC, 16>, 16);
+  if (nv <= 32) return go(k_grad_rows<TY, TG, VEC, 32>, 32);
+  return go(k_grad_rows<TY, TG, VEC, 64>, 64);
+}
+
+template <class TG>
+int launch_join(const Sorted& s, const float* part, int64_t D, float scale, TG* grad,
+                hipStream_t st) {
+  const int vec = D >= 4 ? 4 : 1;
+  const int64_t nv = (D + vec - 1) / vec;
+  hipLaunchKernelGGL((vec == 4 ? k_grad_join<TG, 4> : k_grad_join<TG, 1>),
+                     dim3(kBuckets * kJoinSplit, (unsigned)((nv + 63) / 64)), dim3(kSortThreads), 0,
+                     st, s, part, (int)D, (int)nv, scale, grad);
+  OP_HIP(hipGetLastError(), "g2v_embed_grad");
+  return G2V_OK;
+}
+
+template <class I>
+int launch_sort(const I* ids, int64_t n, int64_t V, int pad, const Plan& p, const Sorted& s,
+                char* ws, hipStream_t st) {
+  if (!p.tiles) {
+    hipLaunchKernelGGL(k_sort_scan<I>, dim3(kBuckets), dim3(kSortThreads), 0, st, ids, n, (int)V,
+                       pad, s);
+  } else {
+    int32_t* counts = reinterpret_cast<int32_t*>(ws + p.counts);
+    int32_t* bfirst = reinterpret_cast<int32_t*>(ws + p.bfirst);
+    int2* pairs = reinterpret_cast<int2*>(ws + p.pairs);
+    hipLaunchKernelGGL(k_tile_count<I>, dim3((unsigned)p.tiles), dim3(kSortThreads), 0, st, ids, n,
+                       p.tile, (int)V, pad, counts);
+    OP_HIP(hipGetLastError(), "g2v_embed_grad");
+    hipLaunchKernelGGL(k_tile_scatter<I>, dim3((unsigned)p.tiles), dim3(kSortThreads), 0, st, ids,
+                       n, p.tile, (int)V, pad, counts, bfirst, pairs);
+    OP_HIP(hipGetLastError(), "g2v_embed_grad");
+    hipLaunchKernelGGL(k_sort_bucket, dim3(kBuckets), dim3(kSortThreads), 0, st, pairs, bfirst,
+                       (int)V, s);
+  }
+  OP_HIP(hipGetLastError(), "g2v_embed_grad");
+  return G2V_OK;
 }
 
 }  // namespace
@@ -153,7 +633,7 @@ extern "C" int g2v_embed_lookup(int device, const void* table, int table_type, i
   g2v::DeviceScope scope(device);
   OP_HIP(scope.error(), what);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  rc = by_type(table_type, [&](auto w) {
+  by_type(table_type, [&](auto w) {
     return by_type(out_type, [&](auto y) {
       return by_id(id_bytes, [&](auto i) {
         using TW = decltype(w);
@@ -162,19 +642,15 @@ extern "C" int g2v_embed_lookup(int device, const void* table, int table_type, i
         constexpr int VEC = vec_of<TW, TY>();
         const int64_t nv = D >= VEC ? (D + VEC - 1) / VEC : D;
         const int64_t blocks = (n * nv + kThreads * kUnits - 1) / (kThreads * kUnits);
-        // a launch is limited to 2^32 threads
-        OP_REQUIRE(blocks < (int64_t)1 << 24, G2V_ERANGE, "%s: %lld x %lld elements in one call",
-                   what, (long long)n, (long long)D);
         hipLaunchKernelGGL((D >= VEC ? k_embed_lookup<TW, TY, I, VEC> : k_embed_lookup<TW, TY, I, 1>),
-                           dim3((unsigned)blocks), dim3(kThreads), 0, st,
+                           grid_of(blocks), dim3(kThreads), 0, st,
                            static_cast<const TW*>(table), V, (int)D, ld,
                            static_cast<const I*>(ids), n * nv, (int)nv, scale,
                            static_cast<TY*>(out));
-        return (int)G2V_OK;
+        return 0;
       });
     });
   });
-  if (rc != G2V_OK) return rc;
   OP_HIP(hipGetLastError(), what);
   return G2V_OK;
 }
@@ -186,6 +662,7 @@ extern "C" int g2v_embed_grad_workspace(int64_t n, int64_t V, int64_t D, int64_t
   const int rc = check_common(what, 0, V, D, nullptr, 4, 0);
   if (rc != G2V_OK) return rc;
   OP_REQUIRE(n >= 0 && n <= INT32_MAX, G2V_ERANGE, "%s: n = %lld", what, (long long)n);
+  *bytes = plan(n, V, D).bytes;
   return G2V_OK;
 }
 
@@ -209,20 +686,26 @@ extern "C" int g2v_embed_grad(int device, const void* dy, int dy_type, int64_t d
   g2v::DeviceScope scope(device);
   OP_HIP(scope.error(), what);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  by_type(dy_type, [&](auto y) {
-    return by_type(grad_type, [&](auto g) {
-      return by_id(id_bytes, [&](auto i) {
-        using TY = decltype(y);
-        using TG = decltype(g);
-        using I = decltype(i);
-        hipLaunchKernelGGL((k_embed_grad_direct<TY, TG, I>),
-                           dim3(grid_for(V * ((D + 63) / 64), kThreads / 64)), dim3(kThreads), 0,
-                           st, static_cast<const TY*>(dy), dy_ld, static_cast<const I*>(ids), n, V,
-                           D, scale, padding_id, static_cast<TG*>(grad));
-        return 0;
-      });
-    });
+  const Plan p = plan(n, V, D);
+  char* ws = static_cast<char*>(workspace);
+  const auto ints = [&](int64_t o) { return reinterpret_cast<int32_t*>(ws + o); };
+  int32_t* small = ints(p.small);
+  const Sorted s{ints(p.perm),  ints(p.start),    ints(p.count),        ints(p.at), ints(p.longs),
+                 small,         small + kBuckets, small + 2 * kBuckets, p.log2L};
+  float* part = reinterpret_cast<float*>(ws + p.part);
+  rc = by_id(id_bytes, [&](auto i) {
+    using I = decltype(i);
+    return launch_sort(static_cast<const I*>(ids), n, V, (int)padding_id, p, s, ws, st);
   });
-  OP_HIP(hipGetLastError(), what);
-  return G2V_OK;
+  if (rc != G2V_OK) return rc;
+  return by_type(grad_type, [&](auto g) {
+    using TG = decltype(g);
+    TG* out = static_cast<TG*>(grad);
+    const int r = by_type(dy_type, [&](auto y) {
+      using TY = decltype(y);
+      return launch_rows<TY, TG, vec_of<TY, TG>()>(static_cast<const TY*>(dy), dy_ld, s, p, part,
+                                                   V, D, scale, out, st);
+    });
+    return r != G2V_OK || p.slots == 0 ? r : launch_join(s, part, D, scale, out, st);
+  });
 }
