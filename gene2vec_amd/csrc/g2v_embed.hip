@@ -73,7 +73,7 @@ __global__ __launch_bounds__(kThreads) void k_embed_lookup(
 #pragma unroll
   for (int k = 0; k < kUnits; ++k)
     if ((int)threadIdx.x + k * kThreads < left)
-      g2v::store_vec<TY, VEC>(out + at[k] * D + col[k], x[k]);
+      g2v::store_vec_nt<TY, VEC>(out + at[k] * D + col[k], x[k]);
 }
 
 // ---- the gradient: tokens sorted by row, then one sum per row --------------------
@@ -86,19 +86,22 @@ __global__ __launch_bounds__(kThreads) void k_embed_lookup(
 // consecutive slices of the tokens, scans the counts and places the tokens.
 //
 // Up to kScanTokens tokens every bucket's workgroup reads all ids itself: it
-// picks its own and counts those of lower buckets, which is where its part of
-// the sorted list begins.  One launch, no exchange between workgroups.  Beyond
-// that the tokens are split into buckets first (tile histograms, then a stable
-// scatter), and every workgroup reads its bucket alone.
+// lists its own in LDS and counts those of lower buckets, which is where its
+// part of the sorted list begins.  One launch, no exchange between workgroups.
+// Beyond that the tokens are split into buckets first (tile counts, then a
+// stable scatter), and every workgroup reads its bucket alone.
 
 constexpr int kBuckets = 256;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / 64;
-constexpr int kKeys = 768;       // rows a bucket counts at a time (48 KB of LDS)
-constexpr int kTileTokens = 8192;
-constexpr int kMaxTiles = 256;   // larger calls take larger tiles
-constexpr int64_t kScanTokens = 65536;
-constexpr int kJoinSplit = 4;    // workgroups per bucket that join long runs
+constexpr int kKeys = 768;          // rows a bucket counts at a time (48 KB of LDS)
+constexpr int kListBits = 10;       // tokens a wave lists: 2^10 (4 KB of LDS)
+constexpr int kScanTokens = kSortWaves << kListBits;
+constexpr int64_t kScanRows = (int64_t)kBuckets << (32 - kListBits);  // a list entry's row
+constexpr int kTileTokens = 1024;
+constexpr int kMaxTiles = 256;      // larger calls take larger tiles
+constexpr int kPer = 2;             // G vectors of a row that one group takes
+constexpr int kJoinBlocks = 512;
 
 struct Sorted {
   int32_t* perm;    // [n] token positions, row by row
@@ -171,13 +174,6 @@ __device__ __forceinline__ int block_scan(int x, int& all) {
   return before + s - x;
 }
 
-// count[key] += the wave's tokens of that key
-__device__ __forceinline__ void count_keys(uint32_t* count, int key, bool has, int bits) {
-  if (!__ballot(has)) return;
-  const uint64_t m = peers(key, has, bits);
-  if (has && __builtin_ctzll(m) == (int)(threadIdx.x & 63)) atomicAdd(&count[key], __popcll(m));
-}
-
 // the place of this lane's token: next[key] plus the lower lanes of that key;
 // next[key] moves on by all of them
 __device__ __forceinline__ int place_keys(uint32_t* next, int key, bool has, int bits) {
@@ -189,39 +185,27 @@ __device__ __forceinline__ int place_keys(uint32_t* next, int key, bool has, int
   return __shfl(old, lead) + __popcll(m & ((1ull << lane) - 1));
 }
 
-// Sorts the tokens of bucket b.  key(i, below): the row of token i over
-// kBuckets, -1 if it is none of b's, below counting the tokens of lower
-// buckets; pos(i): its position.  base: where the bucket begins, less those.
-template <class K, class P>
-__device__ __forceinline__ void sort_bucket(int b, int V, int64_t n, int base, const Sorted& s,
-                                            K key, P pos) {
+// Sorts the tokens of bucket b, which begins at place base.  tokens(f) calls
+// f(position, key) for this wave's tokens of the bucket in order, a whole wave
+// at a time; key: the row over kBuckets, -1 for a lane without a token.
+template <class T>
+__device__ __forceinline__ int sort_bucket(int b, int V, int base, const Sorted& s, T tokens) {
   __shared__ uint32_t hist[kSortWaves * kKeys];
   __shared__ int nlong;
   const int rows = V > b ? (V - b + kBuckets - 1) / kBuckets : 0;
-  uint32_t* mine = hist + (threadIdx.x / 64) * kKeys;
-  int64_t i0, i1;
-  my_slice(n, i0, i1);
-  int first = 0;
-  if (threadIdx.x == 0) nlong = 0;
-  for (int w0 = 0; w0 == 0 || w0 < rows; w0 += kKeys) {
+  const int first = base >> s.log2L, t = threadIdx.x;
+  uint32_t* mine = hist + (t / 64) * kKeys;
+  if (t == 0) nlong = 0;
+  for (int w0 = 0; w0 < rows; w0 += kKeys) {
     const int rw = rows - w0 < kKeys ? rows - w0 : kKeys;
     const int bits = rw > 1 ? 32 - __builtin_clz(rw - 1) : 0;
-    for (int k = threadIdx.x; k < kSortWaves * kKeys; k += kSortThreads) hist[k] = 0;
+    if (t < rw)
+      for (int w = 0; w < kSortWaves; ++w) hist[w * kKeys + t] = 0;
     __syncthreads();
-    int below = 0;
-    for_slice(i0, i1, [&](int64_t i) { return key(i, below); },
-              [&](int64_t, int k) {
-                k -= w0;
-                count_keys(mine, k, k >= 0 && k < rw, bits);
-              });
+    tokens([&](int, int k) {
+      if (k >= w0 && k < w0 + rw) atomicAdd(&mine[k - w0], 1u);
+    });
     __syncthreads();
-    if (w0 == 0) {
-      int all;
-      (void)block_scan(below, all);
-      base += all;
-      first = base >> s.log2L;
-    }
-    const int t = threadIdx.x;
     int c = 0, all;
     if (t < rw)
       for (int w = 0; w < kSortWaves; ++w) c += (int)hist[w * kKeys + t];
@@ -238,24 +222,22 @@ __device__ __forceinline__ void sort_bucket(int b, int V, int64_t n, int base, c
       }
     }
     __syncthreads();
-    for_slice(i0, i1, [&](int64_t i) { int none = 0; return key(i, none); },
-              [&](int64_t i, int k) {
-                const int kw = k - w0;
-                const bool has = kw >= 0 && kw < rw;
-                if (!__ballot(has)) return;
-                const int p = place_keys(mine, kw, has, bits);
-                if (!has) return;
-                s.perm[p] = pos(i);
-                if ((p & ((1 << s.log2L) - 1)) == 0) s.at[p >> s.log2L] = k * kBuckets + b;
-              });
+    tokens([&](int i, int k) {
+      const bool has = k >= w0 && k < w0 + rw;
+      if (!__ballot(has)) return;
+      const int p = place_keys(mine, k - w0, has, bits);
+      if (!has) return;
+      s.perm[p] = i;
+      if ((p & ((1 << s.log2L) - 1)) == 0) s.at[p >> s.log2L] = k * kBuckets + b;
+    });
     base += all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    s.nlong[b] = nlong;
+  if (t == 0) {
+    s.nlong[b] = rows ? nlong : 0;
     s.lfirst[b] = first;
-    if (b == kBuckets - 1) *s.total = base;
   }
+  return base;
 }
 
 // the row of a token, -1 if it names none or the padding
@@ -266,16 +248,36 @@ __device__ __forceinline__ int row_of(const I* __restrict__ ids, int64_t i, int 
 }
 
 template <class I>
-__global__ __launch_bounds__(kSortThreads) void k_sort_scan(const I* __restrict__ ids, int64_t n,
-                                                            int V, int pad, Sorted s) {
-  const int b = blockIdx.x;
-  sort_bucket(b, V, n, 0, s,
-              [&](int64_t i, int& below) {
-                const int v = row_of(ids, i, V, pad), d = v & (kBuckets - 1);
-                below += v >= 0 && d < b;
-                return v >= 0 && d == b ? v / kBuckets : -1;
-              },
-              [](int64_t i) { return (int)i; });
+__global__ __launch_bounds__(kSortThreads) void k_sort_scan(const I* __restrict__ ids, int n, int V,
+                                                            int pad, Sorted s) {
+  __shared__ uint32_t list[kSortWaves << kListBits];  // key << kListBits | position - i0
+  const int b = blockIdx.x, lane = threadIdx.x & 63;
+  int64_t i0, i1;
+  my_slice(n, i0, i1);
+  uint32_t* mine = list + ((threadIdx.x / 64) << kListBits);
+  int below = 0, mine_n = 0;
+  for_slice(i0, i1, [&](int64_t i) { return row_of(ids, i, V, pad); },
+            [&](int64_t i, int v) {
+              const int d = v & (kBuckets - 1);
+              const bool has = v >= 0 && d == b;
+              below += v >= 0 && d < b;
+              const uint64_t m = __ballot(has);
+              if (!m) return;
+              if (has)
+                mine[mine_n + __popcll(m & ((1ull << lane) - 1))] =
+                    (uint32_t)(v / kBuckets) << kListBits | (uint32_t)(i - i0);
+              mine_n += __popcll(m);
+            });
+  int base;
+  (void)block_scan(below, base);
+  const int end = sort_bucket(b, V, base, s, [&](auto f) {
+    for (int j = lane; j - lane < mine_n; j += 64) {
+      const bool in = j < mine_n;
+      const uint32_t e = in ? mine[j] : 0;
+      f((int)i0 + (int)(e & ((1 << kListBits) - 1)), in ? (int)(e >> kListBits) : -1);
+    }
+  });
+  if (b == kBuckets - 1 && threadIdx.x == 0) *s.total = end;
 }
 
 // tokens of every bucket in every tile
@@ -291,7 +293,9 @@ __global__ __launch_bounds__(kSortThreads) void k_tile_count(const I* __restrict
   my_slice(len, i0, i1);
   uint32_t* mine = hist + (threadIdx.x / 64) * kBuckets;
   for_slice(i0, i1, [&](int64_t i) { return row_of(ids, t0 + i, V, pad); },
-            [&](int64_t, int v) { count_keys(mine, v & (kBuckets - 1), v >= 0, 8); });
+            [&](int64_t, int v) {
+              if (v >= 0) atomicAdd(&mine[v & (kBuckets - 1)], 1u);
+            });
   __syncthreads();
   if (threadIdx.x < kBuckets) {
     uint32_t c = 0;
@@ -323,7 +327,9 @@ __global__ __launch_bounds__(kSortThreads) void k_tile_scatter(
   my_slice(len, i0, i1);
   uint32_t* mine = hist + (threadIdx.x / 64) * kBuckets;
   for_slice(i0, i1, [&](int64_t i) { return row_of(ids, t0 + i, V, pad); },
-            [&](int64_t, int v) { count_keys(mine, v & (kBuckets - 1), v >= 0, 8); });
+            [&](int64_t, int v) {
+              if (v >= 0) atomicAdd(&mine[v & (kBuckets - 1)], 1u);
+            });
   before = every = 0;
   if (threadIdx.x < kBuckets)
     for (int q = 0; q < kSortThreads / kBuckets; ++q) {
@@ -357,9 +363,22 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_bucket(const int2* __rest
                                                               const int32_t* __restrict__ bfirst,
                                                               int V, Sorted s) {
   const int b = blockIdx.x, lo = bfirst[b];
-  sort_bucket(b, V, bfirst[b + 1] - lo, lo, s,
-              [&](int64_t i, int&) { return pairs[lo + i].x / kBuckets; },
-              [&](int64_t i) { return pairs[lo + i].y; });
+  int64_t i0, i1;
+  my_slice(bfirst[b + 1] - lo, i0, i1);
+  const int end = sort_bucket(b, V, lo, s, [&](auto f) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t i = i0; i < i1; i += 256) {
+      int2 e[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t j = i + u * 64 + lane;
+        e[u] = j < i1 ? pairs[lo + j] : make_int2(-1, 0);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) f(e[u].y, e[u].x < 0 ? -1 : e[u].x / kBuckets);
+    }
+  });
+  if (b == kBuckets - 1 && threadIdx.x == 0) *s.total = end;
 }
 
 // acc += the rows perm[p0 .. p1) of dy, in that order, eight loads in flight
@@ -387,15 +406,18 @@ __device__ __forceinline__ void sum_rows(const TY* __restrict__ dy, int64_t ld,
   if ((p1 - p0) & 1) some(std::integral_constant<int, 1>{});
 }
 
-// G lanes per row and G vectors of columns: the sum of a row of at most L
-// tokens goes to grad, of none zeros.  A longer run is cut at every L-th of its
-// tokens into pieces for groups of their own, first in the grid as they take
-// longest; their sums go to part.  Pieces are found by place: a run of more
-// than L tokens that begins in [cL, cL + L) covers the place (c + 1) L, and one
-// that begins before cL and has a piece there covers cL.  So slot 2c is the
-// first piece of the run that begins there, slot 2c + 1 a later piece of one
-// that began before; each exists at most once, as two such runs begin more
-// than L places apart.
+// G lanes per row; the sum of a row of at most L tokens goes to grad, of none
+// zeros.  A group takes kPer times G vectors of a row, so that the many rows
+// without a token are written by few groups that live long enough to pay for
+// reading the count.
+//
+// A longer run is cut at every L-th of its tokens into pieces, first in the grid
+// as they take longest and G vectors a group; their sums go to part.  Pieces are
+// found by place: a run of more than L tokens that begins in [cL, cL + L) covers
+// the place (c + 1) L, and one that begins before cL and has a piece there
+// covers cL.  So slot 2c is the first piece of the run that begins there, slot
+// 2c + 1 a later piece of one that began before; each exists at most once, as
+// two such runs begin more than L places apart.
 template <class TY, class TG, int VEC, int G>
 __global__ __launch_bounds__(kThreads) void k_grad_rows(const TY* __restrict__ dy, int64_t ld,
                                                         Sorted s, float* __restrict__ part,
@@ -403,16 +425,16 @@ __global__ __launch_bounds__(kThreads) void k_grad_rows(const TY* __restrict__ d
                                                         int64_t slots, float scale,
                                                         TG* __restrict__ grad) {
   const int64_t it = block_number() * (kThreads / G) + threadIdx.x / G;
-  const int64_t row = tiles == 1 ? it : it / tiles;
-  const int unit = (int)(it - row * tiles) * G + threadIdx.x % G;
-  if (unit >= nv) return;
-  const int col = unit * VEC + VEC <= D ? unit * VEC : D - VEC;
+  const int lane = threadIdx.x % G, L = 1 << s.log2L;
   float acc[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-  const int L = 1 << s.log2L;
-  if (row < slots) {
-    const int c = (int)(row >> 1), later = (int)(row & 1);
+  if (it < slots * tiles) {
+    const int64_t slot = tiles == 1 ? it : it / tiles;
+    const int unit = (int)(it - slot * tiles) * G + lane;
+    if (unit >= nv) return;
+    const int col = unit * VEC + VEC <= D ? unit * VEC : D - VEC;
+    const int c = (int)(slot >> 1), later = (int)(slot & 1);
     const int64_t q = (int64_t)(c + 1 - later) << s.log2L;
     if (q >= *s.total) return;
     const int v = s.at[c + 1 - later], p = s.start[v], n = s.count[v];
@@ -427,37 +449,54 @@ __global__ __launch_bounds__(kThreads) void k_grad_rows(const TY* __restrict__ d
       return;
     }
     sum_rows<TY, VEC>(dy + col, ld, s.perm, p0, p + n - p0 > L ? p0 + L : p + n, acc);
-    g2v::store_vec<float, VEC>(part + row * D + col, acc);
+    g2v::store_vec<float, VEC>(part + slot * D + col, acc);
     return;
   }
-  const int64_t v = row - slots;
+  const int64_t r = it - slots * tiles;
+  const int parts = (tiles + kPer - 1) / kPer;
+  const int64_t v = parts == 1 ? r : r / parts;
   if (v >= V) return;
   const int n = s.count[v];
   if (n > L) return;
-  if (n > 0) {
-    const int p = s.start[v];
-    sum_rows<TY, VEC>(dy + col, ld, s.perm, p, p + n, acc);
-  }
+  const int p = n > 0 ? s.start[v] : 0;
+  int unit = (int)(r - v * parts) * kPer * G + lane;
+  for (int k = 0; k < kPer && unit < nv; ++k, unit += G) {
+    const int col = unit * VEC + VEC <= D ? unit * VEC : D - VEC;
+    if (n > 0) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) acc[i] *= scale;
-  g2v::store_vec<TG, VEC>(grad + v * D + col, acc);
+      for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+      sum_rows<TY, VEC>(dy + col, ld, s.perm, p, p + n, acc);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i] *= scale;
+    }
+    g2v::store_vec_nt<TG, VEC>(grad + v * D + col, acc);
+  }
 }
 
-// a long run's pieces, added in order by kSortWaves waves in turn and those by
-// the first: a workgroup per bucket, share of its long runs, and 64 vectors
+// The pieces of the long runs: kSortWaves waves add every kSortWaves-th piece of
+// a run in order, the first wave those sums.  A workgroup takes 64 vectors of
+// every gridDim.x-th long run; it numbers them itself, bucket by bucket.
 template <class TG, int VEC>
 __global__ __launch_bounds__(kSortThreads) void k_grad_join(Sorted s,
                                                             const float* __restrict__ part, int D,
                                                             int nv, float scale,
                                                             TG* __restrict__ grad) {
   __shared__ float sums[kSortWaves][64][VEC];
-  const int b = blockIdx.x % kBuckets, lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-  const int nlong = s.nlong[b], first = s.lfirst[b];
+  __shared__ int before[kBuckets];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+  int all;
+  const int mine = threadIdx.x < kBuckets ? s.nlong[threadIdx.x] : 0;
+  const int sum = block_scan(mine, all);
+  if (threadIdx.x < kBuckets) before[threadIdx.x] = sum;
+  __syncthreads();
   const int unit = (int)blockIdx.y * 64 + lane;
   const bool in = unit < nv;
   const int col = !in ? 0 : unit * VEC + VEC <= D ? unit * VEC : D - VEC;
-  for (int j = blockIdx.x / kBuckets; j < nlong; j += kJoinSplit) {
-    const int v = s.longs[first + j], n = s.count[v];
+  for (int j = blockIdx.x; j < all; j += gridDim.x) {
+    int b = 0;  // the last bucket with before[b] <= j: it holds run j
+    for (int d = kBuckets / 2; d; d >>= 1)
+      if (before[b + d] <= j) b += d;
+    const int v = s.longs[s.lfirst[b] + j - before[b]], n = s.count[v];
     const int pieces = (n + (1 << s.log2L) - 1) >> s.log2L;
     const int64_t c0 = s.start[v] >> s.log2L;
     float acc[VEC];
@@ -481,7 +520,7 @@ __global__ __launch_bounds__(kSortThreads) void k_grad_join(Sorted s,
         for (int i = 0; i < VEC; ++i) acc[i] += sums[w][lane][i];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) acc[i] *= scale;
-      g2v::store_vec<TG, VEC>(grad + (int64_t)v * D + col, acc);
+      g2v::store_vec_nt<TG, VEC>(grad + (int64_t)v * D + col, acc);
     }
     __syncthreads();
   }
@@ -497,10 +536,14 @@ struct Plan {
 
 Plan plan(int64_t n, int64_t V, int64_t D) {
   Plan p{};
-  p.log2L = n <= 65536 ? 6 : n <= 262144 ? 7 : 8;
+  // short pieces spread a frequent row over more groups, long ones leave less
+  // to join: 65,536 tokens of 24,447 x 200 take 42 us at 64, 43 at 32, 45 at
+  // 128; 262,147 of 60,000 x 512 155 us at 64, 146 at 128, 145 at 256.  A few
+  // hundred tokens are not cut at all, which saves a launch of three.
+  p.log2L = n <= 256 ? 8 : n <= 65536 ? 6 : n <= 262144 ? 7 : 8;
   p.chunks = (n + ((int64_t)1 << p.log2L) - 1) >> p.log2L;
   p.slots = n > (int64_t)1 << p.log2L ? 2 * p.chunks : 0;
-  if (n > kScanTokens) {
+  if (n > kScanTokens || V > kScanRows) {
     p.tile = (n + kMaxTiles - 1) / kMaxTiles;
     p.tile = p.tile < kTileTokens ? kTileTokens : (p.tile + kSortThreads - 1) / kSortThreads * kSortThreads;
     p.tiles = (n + p.tile - 1) / p.tile;
@@ -564,35 +607,43 @@ int check_matrix(const char* what, const char* name, const void* p, int type, in
   return G2V_OK;
 }
 
-template <class TY, class TG, int VEC>
-int launch_rows(const TY* dy, int64_t ld, const Sorted& s, const Plan& p, float* part, int64_t V,
+// f(VEC, G) as constants, for rows of D elements: as few idle lanes as a power
+// of two allows (a row of nv vectors on 64 lanes leaves all but nv without work)
+template <int VEC, class F>
+int by_width(int64_t D, F f) {
+  const int64_t nv = (D + VEC - 1) / VEC;
+  if (D < VEC) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+  const std::integral_constant<int, VEC> vec{};
+  if (nv <= 8) return f(vec, std::integral_constant<int, 8>{});
+  if (nv <= 16) return f(vec, std::integral_constant<int, 16>{});
+  if (nv <= 32) return f(vec, std::integral_constant<int, 32>{});
+  return f(vec, std::integral_constant<int, 64>{});
+}
+
+template <class TY, class TG>
+int launch_rows(const TY* dy, int64_t ld, const Sorted& s, int64_t slots, float* part, int64_t V,
                 int64_t D, float scale, TG* grad, hipStream_t st) {
-  const int64_t nv = D >= VEC ? (D + VEC - 1) / VEC : D;
-  const auto go = [&](auto kernel, int G) {
-    const int64_t tiles = (nv + G - 1) / G;
-    const int64_t blocks = ((p.slots + V) * tiles + kThreads / G - 1) / (kThreads / G);
-    hipLaunchKernelGGL(kernel, grid_of(blocks), dim3(kThreads), 0, st, dy, ld, s, part, V,
-                       (int)D, (int)nv, (int)tiles, p.slots, scale, grad);
+  return by_width<vec_of<TY, TG>()>(D, [&](auto vec, auto g) {
+    constexpr int VEC = decltype(vec)::value, G = decltype(g)::value;
+    const int64_t nv = (D + VEC - 1) / VEC, tiles = (nv + G - 1) / G;
+    const int64_t groups = slots * tiles + V * ((tiles + kPer - 1) / kPer);
+    hipLaunchKernelGGL((k_grad_rows<TY, TG, VEC, G>),
+                       grid_of((groups + kThreads / G - 1) / (kThreads / G)), dim3(kThreads), 0, st,
+                       dy, ld, s, part, V, (int)D, (int)nv, (int)tiles, slots, scale, grad);
     OP_HIP(hipGetLastError(), "g2v_embed_grad");
     return (int)G2V_OK;
-  };
-  // as few idle lanes as a power of two allows: a row of nv vectors on 64
-  // lanes would leave all but nv of them without work
-  if (D < VEC) return go(k_grad_rows<TY, TG, 1, 8>, 8);
-  if (nv <= 8) return go(k_grad_rows<TY, TG, VEC, 8>, 8);
-  if (nv <= 16) return go(k_grad_rows<TY, TG, VEC, 16>, 16);
-  if (nv <= 32) return go(k_grad_rows<TY, TG, VEC, 32>, 32);
-  return go(k_grad_rows<TY, TG, VEC, 64>, 64);
+  });
 }
 
 template <class TG>
-int launch_join(const Sorted& s, const float* part, int64_t D, float scale, TG* grad,
-                hipStream_t st) {
+int launch_join(const Sorted& s, int64_t runs, const float* part, int64_t D, float scale,
+                TG* grad, hipStream_t st) {
   const int vec = D >= 4 ? 4 : 1;
-  const int64_t nv = (D + vec - 1) / vec;
+  const int64_t nv = (D + vec - 1) / vec, cols = (nv + 63) / 64;
+  const int64_t blocks = kJoinBlocks > cols ? kJoinBlocks / cols : 1;
   hipLaunchKernelGGL((vec == 4 ? k_grad_join<TG, 4> : k_grad_join<TG, 1>),
-                     dim3(kBuckets * kJoinSplit, (unsigned)((nv + 63) / 64)), dim3(kSortThreads), 0,
-                     st, s, part, (int)D, (int)nv, scale, grad);
+                     dim3((unsigned)(runs < blocks ? runs : blocks), (unsigned)cols),
+                     dim3(kSortThreads), 0, st, s, part, (int)D, (int)nv, scale, grad);
   OP_HIP(hipGetLastError(), "g2v_embed_grad");
   return G2V_OK;
 }
@@ -601,8 +652,8 @@ template <class I>
 int launch_sort(const I* ids, int64_t n, int64_t V, int pad, const Plan& p, const Sorted& s,
                 char* ws, hipStream_t st) {
   if (!p.tiles) {
-    hipLaunchKernelGGL(k_sort_scan<I>, dim3(kBuckets), dim3(kSortThreads), 0, st, ids, n, (int)V,
-                       pad, s);
+    hipLaunchKernelGGL(k_sort_scan<I>, dim3(kBuckets), dim3(kSortThreads), 0, st, ids, (int)n,
+                       (int)V, pad, s);
   } else {
     int32_t* counts = reinterpret_cast<int32_t*>(ws + p.counts);
     int32_t* bfirst = reinterpret_cast<int32_t*>(ws + p.bfirst);
@@ -686,6 +737,14 @@ extern "C" int g2v_embed_grad(int device, const void* dy, int dy_type, int64_t d
   g2v::DeviceScope scope(device);
   OP_HIP(scope.error(), what);
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  const int pad = (int)padding_id;
+  const auto by_types = [&](auto f) {
+    return by_type(grad_type, [&](auto g) {
+      return by_type(dy_type, [&](auto y) {
+        return f(static_cast<const decltype(y)*>(dy), static_cast<decltype(g)*>(grad));
+      });
+    });
+  };
   const Plan p = plan(n, V, D);
   char* ws = static_cast<char*>(workspace);
   const auto ints = [&](int64_t o) { return reinterpret_cast<int32_t*>(ws + o); };
@@ -695,17 +754,11 @@ extern "C" int g2v_embed_grad(int device, const void* dy, int dy_type, int64_t d
   float* part = reinterpret_cast<float*>(ws + p.part);
   rc = by_id(id_bytes, [&](auto i) {
     using I = decltype(i);
-    return launch_sort(static_cast<const I*>(ids), n, V, (int)padding_id, p, s, ws, st);
+    return launch_sort(static_cast<const I*>(ids), n, V, pad, p, s, ws, st);
   });
   if (rc != G2V_OK) return rc;
-  return by_type(grad_type, [&](auto g) {
-    using TG = decltype(g);
-    TG* out = static_cast<TG*>(grad);
-    const int r = by_type(dy_type, [&](auto y) {
-      using TY = decltype(y);
-      return launch_rows<TY, TG, vec_of<TY, TG>()>(static_cast<const TY*>(dy), dy_ld, s, p, part,
-                                                   V, D, scale, out, st);
-    });
-    return r != G2V_OK || p.slots == 0 ? r : launch_join(s, part, D, scale, out, st);
+  return by_types([&](auto* y, auto* g) {
+    const int r = launch_rows(y, dy_ld, s, p.slots, part, V, D, scale, g, st);
+    return r != G2V_OK || p.slots == 0 ? r : launch_join(s, p.chunks, part, D, scale, g, st);
   });
 }

@@ -11,7 +11,9 @@
 // they are added in a fixed order, so the same gradients give the same bits.
 //
 // The tensors' addresses travel in the kernel arguments, kTensors a launch: no
-// copy to the device, nothing that a captured graph would have to keep alive.
+// copy from the host, nothing that a captured graph would have to keep alive.
+// Longer lists are first written to the workspace by small launches, so that
+// the tensors themselves are always read by one launch, and clipped by one.
 #include <algorithm>
 #include <vector>
 
@@ -23,11 +25,12 @@ using g2v::bf16;
 using g2v::f16;
 
 constexpr int kThreads = 256;
-constexpr int kTensors = 128;      // per launch: 3.6 KB of arguments
-constexpr int kMaxPartials = 2048; // workgroups of all launches, less one a launch
-constexpr int64_t kChunk = 8192;   // elements a workgroup takes at a time
+constexpr int kTensors = 128;       // per launch: 3.7 KB of arguments
+constexpr int kMaxPartials = 2048;  // workgroups: 8 per CU, all resident
+constexpr int64_t kChunk = 8192;    // elements a workgroup takes at a time
+constexpr int kAlign = 64;          // bytes: where a tensor's chunks begin
 
-struct Tensors {
+struct Tensors {  // in the kernel arguments
   const void* src[kTensors];
   void* dst[kTensors];
   int64_t numel[kTensors];
@@ -35,6 +38,41 @@ struct Tensors {
   int8_t type[kTensors];
   int32_t n;
 };
+
+struct TensorList {  // the same in the workspace
+  const void** src;
+  void** dst;
+  int64_t* numel;
+  int32_t* first;
+  int8_t* type;
+  int32_t n;
+};
+
+// A tensor's first chunk also takes the elements before the first aligned
+// address: the rest is read in whole cache lines.
+__host__ __device__ __forceinline__ int64_t head_of(const void* p, int64_t numel, int bytes) {
+  const int64_t h = (int64_t)((0 - (uintptr_t)p) % kAlign) / bytes;
+  return h < numel ? h : numel;
+}
+
+inline int64_t chunks_of(const void* p, int64_t numel, int type) {
+  if (numel == 0) return 0;
+  const int64_t n = numel - head_of(p, numel, (int)g2v::type_bytes(type));
+  return n > kChunk ? (n + kChunk - 1) / kChunk : 1;
+}
+
+__global__ __launch_bounds__(kTensors) void k_list(Tensors a, TensorList to, int at,
+                                                   int chunks_before) {
+  const int t = threadIdx.x;
+  if (t < a.n) {
+    to.src[at + t] = a.src[t];
+    to.dst[at + t] = a.dst[t];
+    to.numel[at + t] = a.numel[t];
+    to.type[at + t] = a.type[t];
+    to.first[at + t + 1] = chunks_before + a.first[t + 1];
+  }
+  if (t == 0 && at == 0) to.first[0] = 0;
+}
 
 template <class F>
 __device__ __forceinline__ void by_type_dev(int type, F f) {
@@ -57,40 +95,18 @@ __device__ __forceinline__ double block_sum(double x) {
   return s;
 }
 
-// calls f(tensor, first element, elements) for the chunks [c0, c1)
-template <class F>
-__device__ __forceinline__ void for_chunks(const Tensors& a, int c0, int c1, F f) {
-  int lo = 0, hi = a.n;  // the tensor of chunk c0: first[lo] <= c0 < first[lo + 1]
-  while (hi - lo > 1) {
-    const int m = (lo + hi) >> 1;
-    if (a.first[m] <= c0) lo = m;
-    else hi = m;
-  }
-  for (int c = c0, t = lo; c < c1; ++c) {
-    while (c >= a.first[t + 1]) ++t;
-    const int64_t e = (int64_t)(c - a.first[t]) * kChunk;
-    const int64_t left = a.numel[t] - e;
-    f(t, e, (int)(left < kChunk ? left : kChunk));
-  }
-}
-
-__device__ __forceinline__ void my_chunks(const Tensors& a, int& c0, int& c1) {
-  const int64_t chunks = a.first[a.n];
-  c0 = (int)(chunks * blockIdx.x / gridDim.x);
-  c1 = (int)(chunks * (blockIdx.x + 1) / gridDim.x);
-}
-
-// x[0 .. n) of p by the workgroup's threads, 16 bytes an access; f(first
-// element, values, their number).  A full chunk is unrolled: all its loads are
-// in flight at once.  The tail goes element by element.
-template <class T, class F>
+// n elements at p by the workgroup, 16 bytes an access: f(first element,
+// values).  A full chunk is unrolled, all its loads in flight at once; a tail
+// goes element by element.
+template <class T, bool NT, class F>
 __device__ __forceinline__ void for_vectors(const T* p, int n, F f) {
   constexpr int VEC = 16 / sizeof(T), kStep = kThreads * VEC;
   if (n == kChunk) {
     float x[kChunk / kStep][VEC];
 #pragma unroll
     for (int k = 0; k < kChunk / kStep; ++k)
-      g2v::load_vec<T, VEC>(p + k * kStep + threadIdx.x * VEC, x[k]);
+      if (NT) g2v::load_vec_nt<T, VEC>(p + k * kStep + threadIdx.x * VEC, x[k]);
+      else g2v::load_vec<T, VEC>(p + k * kStep + threadIdx.x * VEC, x[k]);
 #pragma unroll
     for (int k = 0; k < kChunk / kStep; ++k) f(k * kStep + threadIdx.x * VEC, x[k]);
     return;
@@ -107,23 +123,49 @@ __device__ __forceinline__ void for_vectors(const T* p, int n, F f) {
   }
 }
 
-__global__ __launch_bounds__(kThreads) void k_square_sum(Tensors a, double* __restrict__ partial) {
-  int c0, c1;
-  my_chunks(a, c0, c1);
-  double s0 = 0.0, s1 = 0.0;
-  for_chunks(a, c0, c1, [&](int t, int64_t e, int n) {
+// f(tensor, first element, values) for this workgroup's share of the chunks
+template <bool NT, class A, class F>
+__device__ __forceinline__ void for_elements(const A& a, F f) {
+  const int64_t chunks = a.first[a.n];
+  const int c0 = (int)(chunks * blockIdx.x / gridDim.x);
+  const int c1 = (int)(chunks * (blockIdx.x + 1) / gridDim.x);
+  int lo = 0, hi = a.n;  // the tensor of chunk c0: first[lo] <= c0 < first[lo + 1]
+  while (hi - lo > 1) {
+    const int m = (lo + hi) >> 1;
+    if (a.first[m] <= c0) lo = m;
+    else hi = m;
+  }
+  for (int c = c0, t = lo; c < c1; ++t) {
+    const int t0 = a.first[t], t1 = a.first[t + 1] < c1 ? a.first[t + 1] : c1;
+    const int64_t numel = a.numel[t];
     by_type_dev(a.type[t], [&](auto z) {
       using T = decltype(z);
-      for_vectors(static_cast<const T*>(a.src[t]) + e, n, [&](int, auto& x) {
-        constexpr int N = sizeof x / sizeof x[0];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const double d = (double)x[i];
-          if (i & 1) s1 = fma(d, d, s1);
-          else s0 = fma(d, d, s0);
-        }
-      });
+      const T* p = static_cast<const T*>(a.src[t]);
+      const int head = (int)head_of(p, numel, sizeof(T));
+      if (c == t0 && (int)threadIdx.x < head) {
+        float x[1] = {(float)p[threadIdx.x]};
+        f(t, z, (int64_t)threadIdx.x, x);
+      }
+      for (; c < t1; ++c) {
+        const int64_t e = head + (int64_t)(c - t0) * kChunk, left = numel - e;
+        for_vectors<T, NT>(p + e, (int)(left < kChunk ? left : kChunk),
+                           [&](int i, auto& x) { f(t, z, e + i, x); });
+      }
     });
+  }
+}
+
+template <bool NT, class A>
+__global__ __launch_bounds__(kThreads) void k_square_sum(A a, double* __restrict__ partial) {
+  double s0 = 0.0, s1 = 0.0;
+  for_elements<NT>(a, [&](int, auto, int64_t, auto& x) {
+    constexpr int N = sizeof x / sizeof x[0];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const double d = (double)x[i];
+      if (i & 1) s1 = fma(d, d, s1);
+      else s0 = fma(d, d, s0);
+    }
   });
   const double s = block_sum(s0 + s1);
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
@@ -141,27 +183,25 @@ __global__ __launch_bounds__(kThreads) void k_norm(const double* __restrict__ pa
   if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
-// every workgroup adds the partial sums for itself (the same order, the same
-// factor everywhere): 16 KB from the L2 instead of a launch in between
-__global__ __launch_bounds__(kThreads) void k_clip(Tensors a, const double* __restrict__ partial,
-                                                   int np, double clip, float* __restrict__ norm) {
+// Every workgroup adds the partial sums for itself (the same order, the same
+// factor everywhere): 16 KB from the L2 instead of a launch in between.  What
+// is read here for the last time and what is written go past the caches, and
+// the norm's pass leaves them the gradients: of 400 MB fp32 clipped to another
+// buffer 194 us, 250 with ordinary accesses, 217 with the norm's pass past them.
+template <class A>
+__global__ __launch_bounds__(kThreads) void k_clip(A a, const double* __restrict__ partial, int np,
+                                                   double clip, bool in_place,
+                                                   float* __restrict__ norm) {
   const double nrm = sqrt(sum_partials(partial, np));
-  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nrm;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nrm;
   const float f = (float)(nrm < INFINITY ? clip / (nrm > clip ? nrm : clip) : NAN);
-  int c0, c1;
-  my_chunks(a, c0, c1);
-  for_chunks(a, c0, c1, [&](int t, int64_t e, int n) {
-    if (f == 1.f && a.src[t] == a.dst[t]) return;  // in place and within the bound
-    by_type_dev(a.type[t], [&](auto z) {
-      using T = decltype(z);
-      T* q = static_cast<T*>(a.dst[t]) + e;
-      for_vectors(static_cast<const T*>(a.src[t]) + e, n, [&](int at, auto& x) {
-        constexpr int N = sizeof x / sizeof x[0];
+  if (in_place && f == 1.f) return;  // within the bound
+  for_elements<true>(a, [&](int t, auto z, int64_t at, auto& x) {
+    using T = decltype(z);
+    constexpr int N = sizeof x / sizeof x[0];
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] *= f;
-        g2v::store_vec<T, N>(q + at, x);
-      });
-    });
+    for (int i = 0; i < N; ++i) x[i] *= f;
+    g2v::store_vec_nt<T, N>(static_cast<T*>(a.dst[t]) + at, x);
   });
 }
 
@@ -193,7 +233,7 @@ int check_list(const char* what, int device, const void* const* src, const int64
                (long long)numel[t]);
     OP_REQUIRE(numel[t] == 0 || (src[t] && (uintptr_t)src[t] % b == 0), G2V_EINVAL,
                "%s: tensor %lld is null or not aligned to its type", what, (long long)t);
-    chunks += (numel[t] + kChunk - 1) / kChunk;
+    chunks += chunks_of(src[t], numel[t], types[t]);
     OP_REQUIRE(chunks <= INT32_MAX, G2V_ERANGE, "%s: more than 2^44 elements in all", what);
   }
   return G2V_OK;
@@ -232,57 +272,77 @@ int check_apart(const char* what, const void* const* src, void* const* dst, cons
   return G2V_OK;
 }
 
-// f(arguments, workgroups, is it the first) for every kTensors tensors that
-// hold something; the workgroups of all calls are at most kMaxPartials + calls
+// where the parts of the workspace lie: partial sums, then the list where it
+// does not fit the kernel arguments
+struct Plan {
+  int64_t src, dst, numel, first, type, bytes;
+};
+
+Plan plan(int64_t n) {
+  Plan p{};
+  const auto take = [&](int64_t count, int64_t size) {
+    const int64_t o = p.bytes;
+    p.bytes += (count * size + 15) / 16 * 16;
+    return o;
+  };
+  take(kMaxPartials, sizeof(double));
+  const int64_t k = n > kTensors ? n : 0;
+  p.src = take(k, 8);
+  p.dst = take(k, 8);
+  p.numel = take(k, 8);
+  p.first = take(k + 1, 4);
+  p.type = take(k, 1);
+  return p;
+}
+
+// f(the list as a kernel takes it, workgroups), once; not at all for a list
+// that holds no element
 template <class F>
-int for_launches(const void* const* src, void* const* dst, const int64_t* numel,
-                 const int32_t* types, int64_t n, F f) {
-  int64_t total = 0;
-  for (int64_t t = 0; t < n; ++t) total += (numel[t] + kChunk - 1) / kChunk;
-  bool first = true;
+int with_tensors(const void* const* src, void* const* dst, const int64_t* numel,
+                 const int32_t* types, int64_t n, char* ws, hipStream_t st, F f) {
+  int64_t full = 0;
+  for (int64_t t = 0; t < n; ++t) full += numel[t] > 0;
+  if (full == 0) return G2V_OK;
+  const Plan p = plan(n);
+  const TensorList list{reinterpret_cast<const void**>(ws + p.src),
+                        reinterpret_cast<void**>(ws + p.dst),
+                        reinterpret_cast<int64_t*>(ws + p.numel),
+                        reinterpret_cast<int32_t*>(ws + p.first),
+                        reinterpret_cast<int8_t*>(ws + p.type), (int32_t)full};
   Tensors a;
   a.n = 0;
   a.first[0] = 0;
+  int64_t listed = 0, chunks = 0;
   for (int64_t t = 0; t < n; ++t) {
-    if (numel[t] > 0) {
-      a.src[a.n] = src[t];
-      a.dst[a.n] = dst ? dst[t] : nullptr;
-      a.numel[a.n] = numel[t];
-      a.type[a.n] = (int8_t)types[t];
-      a.first[a.n + 1] = a.first[a.n] + (int32_t)((numel[t] + kChunk - 1) / kChunk);
-      ++a.n;
-    }
-    if (a.n == kTensors || (t == n - 1 && a.n > 0)) {
-      const int64_t c = a.first[a.n];
-      const int64_t g = total <= kMaxPartials ? c : (c * kMaxPartials + total - 1) / total;
-      f(a, (unsigned)g, first);
-      const hipError_t e = hipGetLastError();
-      if (e != hipSuccess) return g2v::op_fail(G2V_EHIP, "launch: %s", hipGetErrorString(e));
-      first = false;
+    if (numel[t] == 0) continue;
+    a.src[a.n] = src[t];
+    a.dst[a.n] = dst ? dst[t] : nullptr;
+    a.numel[a.n] = numel[t];
+    a.type[a.n] = (int8_t)types[t];
+    a.first[a.n + 1] = a.first[a.n] + (int32_t)chunks_of(src[t], numel[t], types[t]);
+    ++a.n;
+    if (full > kTensors && (a.n == kTensors || listed + a.n == full)) {
+      hipLaunchKernelGGL(k_list, dim3(1), dim3(kTensors), 0, st, a, list, (int)listed, (int)chunks);
+      OP_HIP(hipGetLastError(), "g2v_global_norm");
+      listed += a.n;
+      chunks += a.first[a.n];
       a.n = 0;
     }
   }
+  if (full <= kTensors) chunks = a.first[a.n];
+  const unsigned g = (unsigned)(chunks < kMaxPartials ? chunks : kMaxPartials);
+  if (full <= kTensors) f(a, g);
+  else f(list, g);
+  OP_HIP(hipGetLastError(), "g2v_global_norm");
   return G2V_OK;
-}
-
-int square_sums(const void* const* src, const int64_t* numel, const int32_t* types, int64_t n,
-                double* partial, int* np, hipStream_t st) {
-  int used = 0;
-  const int rc = for_launches(src, nullptr, numel, types, n,
-                              [&](const Tensors& a, unsigned g, bool) {
-                                hipLaunchKernelGGL(k_square_sum, dim3(g), dim3(kThreads), 0, st, a,
-                                                   partial + used);
-                                used += (int)g;
-                              });
-  *np = used;
-  return rc;
 }
 
 }  // namespace
 
 extern "C" int g2v_global_norm_workspace(int64_t n, int64_t* bytes) {
   OP_REQUIRE(bytes && n >= 0, G2V_EINVAL, "g2v_global_norm_workspace: bad arguments");
-  *bytes = (int64_t)sizeof(double) * (kMaxPartials + 1 + n / kTensors + 1);
+  OP_REQUIRE(n <= INT32_MAX, G2V_ERANGE, "g2v_global_norm_workspace: %lld tensors", (long long)n);
+  *bytes = plan(n).bytes;
   return G2V_OK;
 }
 
@@ -296,8 +356,20 @@ extern "C" int g2v_global_norm(int device, const void* const* tensors, const int
   OP_HIP(scope.error(), what);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   double* partial = static_cast<double*>(workspace);
+  // beyond the Infinity Cache's 256 MB nothing stays for the next reader, and
+  // loads past the caches are faster (1 GB of fp32: 167 us against 190); what
+  // fits may still lie there (200 MB: 38 us against 35)
+  double bytes = 0.0;
+  for (int64_t t = 0; t < n; ++t) bytes += (double)(numel[t] * g2v::type_bytes(types[t]));
+  const bool large = bytes > 256e6;
   int np = 0;
-  rc = square_sums(tensors, numel, types, n, partial, &np, st);
+  rc = with_tensors(tensors, nullptr, numel, types, n, static_cast<char*>(workspace), st,
+                    [&](const auto& a, unsigned g) {
+                      using A = std::decay_t<decltype(a)>;
+                      hipLaunchKernelGGL((large ? k_square_sum<true, A> : k_square_sum<false, A>),
+                                         dim3(g), dim3(kThreads), 0, st, a, partial);
+                      np = (int)g;
+                    });
   if (rc != G2V_OK) return rc;
   hipLaunchKernelGGL(k_norm, dim3(1), dim3(kThreads), 0, st, partial, np, norm);
   OP_HIP(hipGetLastError(), what);
@@ -320,20 +392,25 @@ extern "C" int g2v_clip_global_norm(int device, const void* const* src, void* co
     return g2v::op_fail(G2V_ENOMEM, "%s: no host memory for %lld tensors", what, (long long)n);
   }
   if (rc != G2V_OK) return rc;
+  bool in_place = true;
+  for (int64_t t = 0; t < n; ++t) in_place = in_place && (numel[t] == 0 || src[t] == dst[t]);
   g2v::DeviceScope scope(device);
   OP_HIP(scope.error(), what);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   double* partial = static_cast<double*>(workspace);
-  int np = 0;
-  rc = square_sums(src, numel, types, n, partial, &np, st);
-  if (rc != G2V_OK) return rc;
-  if (np == 0) {  // nothing to clip: the norm of nothing is 0
-    hipLaunchKernelGGL(k_norm, dim3(1), dim3(kThreads), 0, st, partial, 0, norm);
-    OP_HIP(hipGetLastError(), what);
-    return G2V_OK;
-  }
-  return for_launches(src, dst, numel, types, n, [&](const Tensors& a, unsigned g, bool first) {
-    hipLaunchKernelGGL(k_clip, dim3(g), dim3(kThreads), 0, st, a, partial, np, clip_norm,
-                       first ? norm : nullptr);
-  });
+  bool any = false;
+  rc = with_tensors(src, dst, numel, types, n, static_cast<char*>(workspace), st,
+                    [&](const auto& a, unsigned g) {
+                      using A = std::decay_t<decltype(a)>;
+                      hipLaunchKernelGGL((k_square_sum<false, A>), dim3(g), dim3(kThreads), 0, st,
+                                         a, partial);
+                      hipLaunchKernelGGL(k_clip<A>, dim3(g), dim3(kThreads), 0, st, a, partial,
+                                         (int)g, clip_norm, in_place, norm);
+                      any = true;
+                    });
+  if (rc != G2V_OK || any) return rc;
+  // nothing to clip: the norm of nothing is 0
+  hipLaunchKernelGGL(k_norm, dim3(1), dim3(kThreads), 0, st, partial, 0, norm);
+  OP_HIP(hipGetLastError(), what);
+  return G2V_OK;
 }

@@ -6,6 +6,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "g2v.h"
 #include "g2v_internal.h"
 
@@ -32,6 +34,44 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[VEC]) {
 #pragma unroll
   for (int i = 0; i < VEC; ++i) t[i] = (T)x[i];
   __builtin_memcpy(p, t, sizeof t);
+}
+
+typedef uint32_t word4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t word4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// the same, past the caches: for results larger than they hold
+template <class T, int VEC>
+__device__ __forceinline__ void store_vec_nt(T* p, const float (&x)[VEC]) {
+  if constexpr (sizeof(T) * VEC % 16 == 0) {
+    using word4 = std::conditional_t<sizeof(T) == 2, word4_at2, word4_at4>;
+    T t[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) t[i] = (T)x[i];
+    word4 w[sizeof(T) * VEC / 16];
+    __builtin_memcpy(w, t, sizeof t);
+#pragma unroll
+    for (unsigned k = 0; k < sizeof(T) * VEC / 16; ++k)
+      __builtin_nontemporal_store(w[k], reinterpret_cast<word4*>(p) + k);
+  } else {
+    store_vec<T, VEC>(p, x);
+  }
+}
+
+template <class T, int VEC>
+__device__ __forceinline__ void load_vec_nt(const T* p, float (&x)[VEC]) {
+  if constexpr (sizeof(T) * VEC % 16 == 0) {
+    using word4 = std::conditional_t<sizeof(T) == 2, word4_at2, word4_at4>;
+    word4 w[sizeof(T) * VEC / 16];
+#pragma unroll
+    for (unsigned k = 0; k < sizeof(T) * VEC / 16; ++k)
+      w[k] = __builtin_nontemporal_load(reinterpret_cast<const word4*>(p) + k);
+    T t[VEC];
+    __builtin_memcpy(t, w, sizeof t);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = (float)t[i];
+  } else {
+    load_vec<T, VEC>(p, x);
+  }
 }
 
 inline int64_t type_bytes(int type) {

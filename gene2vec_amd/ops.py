@@ -25,7 +25,9 @@ from __future__ import annotations
 
 import array
 import ctypes as C
+import functools
 import math
+from operator import attrgetter
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -37,92 +39,104 @@ _ID_BYTES = {torch.int32: 4, torch.int64: 8}
 _FLT_MAX = torch.finfo(torch.float32).max
 
 
-def _refuse(cond, msg):
-    if cond:
-        raise ValueError(msg)
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _workspace(nbytes, device):
-    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+def _stream(index):
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _on_gpu(t, name):
-    _refuse(not isinstance(t, torch.Tensor), f"{name} must be a tensor, not {type(t).__name__}")
-    _refuse(t.layout is not torch.strided or not t.is_cuda,
-            f"{name} must be a dense tensor on the GPU (there is no CPU fallback)")
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor, not {type(t).__name__}")
+    if not t.is_cuda or t.layout is not torch.strided:
+        raise ValueError(f"{name} must be a dense tensor on the GPU (there is no CPU fallback)")
 
 
 def _check_ids(ids, device):
     _on_gpu(ids, "ids")
-    _refuse(ids.dtype not in _ID_BYTES, f"ids must be int32 or int64, not {ids.dtype}")
-    _refuse(ids.device != device, f"ids are on {ids.device}, the rows on {device}")
+    if ids.dtype not in _ID_BYTES:
+        raise ValueError(f"ids must be int32 or int64, not {ids.dtype}")
+    if ids.device != device:
+        raise ValueError(f"ids are on {ids.device}, the rows on {device}")
 
 
 def _check_options(scale, padding_idx, V, dtype):
     scale = float(scale)
-    _refuse(not abs(scale) <= _FLT_MAX, f"scale must be finite in fp32, not {scale}")
-    _refuse(dtype not in _TYPES, f"dtype must be float32, float16 or bfloat16, not {dtype}")
+    if not abs(scale) <= _FLT_MAX:
+        raise ValueError(f"scale must be finite in fp32, not {scale}")
+    if dtype not in _TYPES:
+        raise ValueError(f"dtype must be float32, float16 or bfloat16, not {dtype}")
     if padding_idx is None:
         return scale, -1
     pad = int(padding_idx)
-    _refuse(pad != padding_idx or not 0 <= pad < V, f"padding_idx {padding_idx} is not in [0, {V})")
+    if pad != padding_idx or not 0 <= pad < V:
+        raise ValueError(f"padding_idx {padding_idx} is not in [0, {V})")
     return scale, pad
 
 
-def _row_stride(t, name):
-    """the row stride of a matrix whose rows are contiguous"""
-    V, D = t.shape
-    _refuse(D > 1 and t.stride(1) != 1, f"the elements of a row of {name} must be contiguous")
-    ld = t.stride(0) if V > 1 else D
-    _refuse(ld < D, f"the rows of {name} overlap (strides {tuple(t.stride())})")
-    return ld
+def _row_stride(t, V, D):
+    """the row stride of the table, whose rows are contiguous"""
+    s0, s1 = t.stride()
+    if s1 != 1 and D > 1:
+        raise ValueError("the elements of a row of params must be contiguous")
+    if V == 1:
+        return D
+    if s0 < D:
+        raise ValueError(f"the rows of params overlap (strides {t.stride()})")
+    return s0
 
 
-def _lookup(params, ids, scale, dtype):
+def _lookup(params, ids, ld, scale, dtype):
     V, D = params.shape
-    out = torch.empty(ids.shape + (D,), dtype=dtype, device=params.device)
-    ids = ids.contiguous()
+    index = params.device.index
+    out = params.new_empty(ids.shape + (D,), dtype=dtype)
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
     N.check(N.lib().g2v_embed_lookup(
-        params.device.index, params.data_ptr(), _TYPES[params.dtype], V, D,
-        _row_stride(params, "params"), ids.data_ptr(), _ID_BYTES[ids.dtype], ids.numel(), scale,
-        out.data_ptr(), _TYPES[dtype], _stream(params.device)))
+        index, params.data_ptr(), _TYPES[params.dtype], V, D, ld, ids.data_ptr(),
+        _ID_BYTES[ids.dtype], ids.numel(), scale, out.data_ptr(), _TYPES[dtype], _stream(index)))
     return out
 
 
-def _lookup_grad(dy, ids, V, D, scale, pad, dtype):
-    ids = ids.contiguous()
-    n = ids.numel()
-    dy = dy.reshape(n, D)
-    if (D > 1 and dy.stride(1) != 1) or (n > 1 and dy.stride(0) < D):
-        dy = dy.contiguous()  # a transposed or broadcast gradient
+@functools.lru_cache(maxsize=256)
+def _grad_workspace(n, V, D):
     nbytes = C.c_int64()
     N.check(N.lib().g2v_embed_grad_workspace(n, V, D, C.byref(nbytes)))
-    grad = torch.empty(V, D, dtype=dtype, device=dy.device)
-    ws = _workspace(nbytes.value, dy.device)
+    return nbytes.value
+
+
+def _lookup_grad(dy, ids, V, D, scale, pad, dtype):
+    n = ids.numel()
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
+    if dy.dim() != 2:
+        dy = dy.reshape(n, D)
+    ld, s1 = dy.stride()
+    if n <= 1:
+        ld = D
+    if (s1 != 1 and D > 1) or ld < D:  # a transposed or broadcast gradient
+        dy = dy.contiguous()
+        ld = D
+    index = dy.device.index
+    nbytes = _grad_workspace(n, V, D)
+    grad = dy.new_empty((V, D), dtype=dtype)
+    ws = dy.new_empty(nbytes, dtype=torch.uint8)
     N.check(N.lib().g2v_embed_grad(
-        dy.device.index, dy.data_ptr(), _TYPES[dy.dtype], dy.stride(0) if n > 1 else D,
-        ids.data_ptr(), _ID_BYTES[ids.dtype], n, V, D, scale, pad, grad.data_ptr(), _TYPES[dtype],
-        ws.data_ptr(), ws.numel(), _stream(dy.device)))
+        index, dy.data_ptr(), _TYPES[dy.dtype], ld, ids.data_ptr(), _ID_BYTES[ids.dtype], n, V, D,
+        scale, pad, grad.data_ptr(), _TYPES[dtype], ws.data_ptr(), nbytes, _stream(index)))
     return grad
 
 
 class _EmbeddingLookup(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, params, ids, scale, pad, dtype):
+    def forward(ctx, params, ids, ld, scale, pad, dtype):
         ctx.save_for_backward(ids)
-        ctx.args = params.shape[0], params.shape[1], scale, pad, params.dtype
-        return _lookup(params, ids, scale, dtype)
+        ctx.args = *params.shape, scale, pad, params.dtype
+        return _lookup(params, ids, ld, scale, dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         ids, = ctx.saved_tensors
-        V, D, scale, pad, dtype = ctx.args
-        return _lookup_grad(dy, ids, V, D, scale, pad, dtype), None, None, None, None
+        return _lookup_grad(dy, ids, *ctx.args), None, None, None, None, None
 
 
 def embedding_lookup(params, ids, scale=1.0, padding_idx=None, dtype=None):
@@ -141,17 +155,19 @@ def embedding_lookup(params, ids, scale=1.0, padding_idx=None, dtype=None):
     copied.
     """
     _on_gpu(params, "params")
-    _refuse(params.dim() != 2 or params.numel() == 0,
-            f"params must be a matrix [V, D], not {tuple(params.shape)}")
-    _refuse(params.dtype not in _TYPES,
-            f"params must be float32, float16 or bfloat16, not {params.dtype}")
-    _row_stride(params, "params")
+    if params.dim() != 2 or params.numel() == 0:
+        raise ValueError(f"params must be a matrix [V, D], not {tuple(params.shape)}")
+    if params.dtype not in _TYPES:
+        raise ValueError(f"params must be float32, float16 or bfloat16, not {params.dtype}")
+    V, D = params.shape
+    ld = _row_stride(params, V, D)
     _check_ids(ids, params.device)
-    dtype = params.dtype if dtype is None else dtype
-    scale, pad = _check_options(scale, padding_idx, params.shape[0], dtype)
+    if dtype is None:
+        dtype = params.dtype
+    scale, pad = _check_options(scale, padding_idx, V, dtype)
     if params.requires_grad and torch.is_grad_enabled():
-        return _EmbeddingLookup.apply(params, ids, scale, pad, dtype)
-    return _lookup(params, ids, scale, dtype)
+        return _EmbeddingLookup.apply(params, ids, ld, scale, pad, dtype)
+    return _lookup(params, ids, ld, scale, dtype)
 
 
 def embedding_lookup_grad(dy, ids, vocab_size, scale=1.0, padding_idx=None, dtype=None):
@@ -164,11 +180,14 @@ def embedding_lookup_grad(dy, ids, vocab_size, scale=1.0, padding_idx=None, dtyp
     """
     _on_gpu(dy, "dy")
     _check_ids(ids, dy.device)
-    _refuse(dy.dtype not in _TYPES, f"dy must be float32, float16 or bfloat16, not {dy.dtype}")
-    _refuse(dy.dim() != ids.dim() + 1 or dy.shape[:-1] != ids.shape or dy.shape[-1] < 1,
-            f"dy {tuple(dy.shape)} does not hold a row for each of ids {tuple(ids.shape)}")
+    if dy.dtype not in _TYPES:
+        raise ValueError(f"dy must be float32, float16 or bfloat16, not {dy.dtype}")
+    if dy.dim() != ids.dim() + 1 or dy.shape[:-1] != ids.shape or dy.shape[-1] < 1:
+        raise ValueError(f"dy {tuple(dy.shape)} does not hold a row for each of ids "
+                         f"{tuple(ids.shape)}")
     V = int(vocab_size)
-    _refuse(V != vocab_size or V < 1, f"vocab_size must be a positive number, not {vocab_size}")
+    if V != vocab_size or V < 1:
+        raise ValueError(f"vocab_size must be a positive number, not {vocab_size}")
     dtype = dy.dtype if dtype is None else dtype
     scale, pad = _check_options(scale, padding_idx, V, dtype)
     return _lookup_grad(dy.detach(), ids, V, dy.shape[-1], scale, pad, dtype)
@@ -190,22 +209,29 @@ def _check_list(t_list, what):
     """the tensors of the list that are there, and their device"""
     t_list = list(t_list)
     there = [t for t in t_list if t is not None]
-    _refuse(not there, f"{what}: the list holds no tensor")
-    device = there[0].device if isinstance(there[0], torch.Tensor) else None
-    grad = torch.is_grad_enabled()
+    if not there:
+        raise ValueError(f"{what}: the list holds no tensor")
     for t in there:
-        if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.device != device
-                or t.dtype not in _TYPES or t.layout is not torch.strided
-                or (grad and t.requires_grad) or not _is_dense(t)):
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{what}: the list must hold tensors, not {type(t).__name__}")
+    devices = set(map(attrgetter("device"), there))
+    if (len(devices) > 1 or not there[0].is_cuda
+            or set(map(attrgetter("layout"), there)) != {torch.strided}):
+        for t in there:
             _on_gpu(t, what)
-            _refuse(t.device != device, f"{what}: tensors on {device} and {t.device}")
-            _refuse(t.dtype not in _TYPES,
-                    f"{what}: tensors must be float32, float16 or bfloat16, not {t.dtype}")
-            _refuse(grad and t.requires_grad,
-                    f"{what} is not differentiable: pass gradients, or call it under no_grad()")
-            _refuse(True, f"{what}: the elements of a tensor must be dense in memory "
-                          f"(shape {tuple(t.shape)}, strides {tuple(t.stride())})")
-    return t_list, there, device
+        raise ValueError(f"{what}: tensors on {sorted(map(str, devices))}")
+    if not set(map(attrgetter("dtype"), there)) <= _TYPES.keys():
+        raise ValueError(f"{what}: tensors must be float32, float16 or bfloat16, not "
+                         f"{sorted({str(t.dtype) for t in there})}")
+    if torch.is_grad_enabled() and any(map(attrgetter("requires_grad"), there)):
+        raise ValueError(f"{what} is not differentiable: pass gradients, or call it under "
+                         "no_grad()")
+    if not all(map(torch.Tensor.is_contiguous, there)):
+        for t in there:
+            if not _is_dense(t):
+                raise ValueError(f"{what}: the elements of a tensor must be dense in memory "
+                                 f"(shape {tuple(t.shape)}, strides {t.stride()})")
+    return t_list, there, devices.pop()
 
 
 def _address(a):
@@ -213,16 +239,21 @@ def _address(a):
 
 
 def _pointers(tensors):
-    return array.array("Q", [t.data_ptr() for t in tensors])
+    return array.array("Q", map(torch.Tensor.data_ptr, tensors))
 
 
-def _describe(there, device):
-    numel = array.array("q", [t.numel() for t in there])
-    types = array.array("i", [_TYPES[t.dtype] for t in there])
+@functools.lru_cache(maxsize=256)
+def _norm_workspace(n):
     nbytes = C.c_int64()
-    N.check(N.lib().g2v_global_norm_workspace(len(there), C.byref(nbytes)))
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    return numel, types, norm, _workspace(nbytes.value, device)
+    N.check(N.lib().g2v_global_norm_workspace(n, C.byref(nbytes)))
+    return nbytes.value
+
+
+def _describe(there):
+    numel = array.array("q", map(torch.Tensor.numel, there))
+    types = array.array("i", [_TYPES[t.dtype] for t in there])
+    norm = there[0].new_empty((), dtype=torch.float32)
+    return numel, types, norm, there[0].new_empty(_norm_workspace(len(there)), dtype=torch.uint8)
 
 
 def global_norm(t_list):
@@ -235,32 +266,28 @@ def global_norm(t_list):
     """
     _, there, device = _check_list(t_list, "global_norm")
     src = _pointers(there)
-    numel, types, norm, ws = _describe(there, device)
+    numel, types, norm, ws = _describe(there)
     N.check(N.lib().g2v_global_norm(device.index, _address(src), _address(numel), _address(types),
                                     len(there), norm.data_ptr(), ws.data_ptr(), ws.numel(),
-                                    _stream(device)))
+                                    _stream(device.index)))
     return norm
 
 
 def _clip(there, outs, device, clip_norm):
     clip_norm = float(clip_norm)
-    _refuse(not 0.0 < clip_norm < math.inf,
-            f"clip_norm must be positive and finite, not {clip_norm}")
+    if not 0.0 < clip_norm < math.inf:
+        raise ValueError(f"clip_norm must be positive and finite, not {clip_norm}")
     src = _pointers(there)
     dst = src if outs is there else _pointers(outs)
-    numel, types, norm, ws = _describe(there, device)
+    numel, types, norm, ws = _describe(there)
     try:
         N.check(N.lib().g2v_clip_global_norm(
             device.index, _address(src), _address(dst), _address(numel), _address(types),
-            len(there), clip_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(), _stream(device)))
-    except N.G2VError as e:
+            len(there), clip_norm, norm.data_ptr(), ws.data_ptr(), ws.numel(),
+            _stream(device.index)))
+    except N.G2VError as e:  # tensors that overlap
         raise (ValueError(str(e)) if e.code == N.G2V_EINVAL else e)
     return norm
-
-
-def _written(tensors):
-    """autograd learns that they changed"""
-    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
 
 
 def clip_by_global_norm(t_list, clip_norm, out=None):
@@ -279,22 +306,19 @@ def clip_by_global_norm(t_list, clip_norm, out=None):
         outs = [o for o in out if o is not None]
     else:
         out = list(out)
-        _refuse(len(out) != len(t_list),
-                f"clip_by_global_norm: {len(out)} outputs for {len(t_list)} tensors")
-        outs = []
-        for t, o in zip(t_list, out):
-            if t is None:
-                continue
+        if len(out) != len(t_list):
+            raise ValueError(f"clip_by_global_norm: {len(out)} outputs for {len(t_list)} tensors")
+        outs = [o for t, o in zip(t_list, out) if t is not None]
+        for t, o in zip(there, outs):
             _on_gpu(o, "clip_by_global_norm: out")
-            _refuse(o.shape != t.shape or o.dtype != t.dtype or o.device != t.device
-                    or not (o.is_contiguous() and t.is_contiguous() or o.stride() == t.stride()),
-                    "clip_by_global_norm: an output differs from its tensor in shape, type, "
-                    "strides or device")
-            _refuse(torch.is_grad_enabled() and o.requires_grad,
-                    "clip_by_global_norm: an output requires a gradient")
-            outs.append(o)
+            if (o.shape != t.shape or o.dtype != t.dtype or o.device != device
+                    or not (o.is_contiguous() and t.is_contiguous() or o.stride() == t.stride())):
+                raise ValueError("clip_by_global_norm: an output differs from its tensor in "
+                                 "shape, type, strides or device")
+            if o.requires_grad and torch.is_grad_enabled():
+                raise ValueError("clip_by_global_norm: an output requires a gradient")
     norm = _clip(there, outs, device, clip_norm)
-    _written(outs)
+    torch.autograd.graph.increment_version(outs)
     return [None if t is None else o for t, o in zip(t_list, out)], norm
 
 
@@ -302,5 +326,5 @@ def clip_by_global_norm_(t_list, clip_norm):
     """``clip_by_global_norm`` in place; returns the norm before it."""
     _, there, device = _check_list(t_list, "clip_by_global_norm_")
     norm = _clip(there, there, device, clip_norm)
-    _written(there)
+    torch.autograd.graph.increment_version(there)
     return norm
