@@ -142,8 +142,42 @@ def build(force: bool = False, verbose: bool = False, ablations: bool = False,
     return out
 
 
+TORCH_LIB = os.path.join(HERE, "_g2v_torch.so")
+TORCH_SOURCE = os.path.join(CSRC, "g2v_torch.cpp")
+
+
+def build_torch(force: bool = False, verbose: bool = False) -> str:
+    """the operators' Python module (_g2v_torch.so): host code against the
+    installed torch and libg2v.so, which is built before"""
+    deps = (TORCH_SOURCE, os.path.join(ROOT, "include", "g2v.h"), __file__)
+    if (not force and os.path.exists(TORCH_LIB)
+            and all(os.path.getmtime(d) <= os.path.getmtime(TORCH_LIB) for d in deps)):
+        return TORCH_LIB
+    import sysconfig
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    rocm = os.path.dirname(os.path.dirname(hipcc()))
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-pthread", "-fvisibility=hidden",
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", os.path.join(ROOT, "include"),
+           *(f"-isystem{d}" for d in (*include_paths(), sysconfig.get_paths()["include"],
+                                      os.path.join(rocm, "include"))),
+           TORCH_SOURCE, "-L", HERE, "-lg2v", *(f"-L{d}" for d in library_paths()),
+           "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_hip", "-lc10",
+           "-Wl,-rpath,$ORIGIN", "-o", TORCH_LIB + ".tmp"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode:
+        raise RuntimeError(f"g++ failed on {TORCH_SOURCE}:\n{r.stderr}")
+    os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+    return TORCH_LIB
+
+
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose=True, ablations="--ablations" in sys.argv))
+    print(build_torch(force="--force" in sys.argv, verbose=True))
 
 
 EXAMPLES = os.path.join(os.path.dirname(HERE), "examples")

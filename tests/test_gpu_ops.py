@@ -261,6 +261,34 @@ def test_two_lookups_of_one_table_accumulate():
     check_grad(w.grad, torch.cat([ca, cb]), torch.cat([a, b]), 50)
 
 
+def test_inference_mode():
+    w = torch.randn(20, 8, device="cuda", requires_grad=True)
+    ids = torch.arange(20, device="cuda")
+    with torch.inference_mode():
+        y = ops.embedding_lookup(w, ids)
+        outs, norm = ops.clip_by_global_norm([y], 0.1)
+        ops.clip_by_global_norm_([y], 0.1)
+        assert torch.equal(outs[0], y) and float(norm) > 0.1
+    assert y.is_inference() and not y.requires_grad
+    assert float(ops.global_norm([y])) > 0
+    with pytest.raises(ValueError, match="inference"):
+        ops.clip_by_global_norm_([y], 0.1)
+
+
+def test_grad_modes_and_a_computed_table():
+    w = torch.randn(20, 8, device="cuda")
+    ids = torch.arange(6, device="cuda")
+    assert not ops.embedding_lookup(w, ids).requires_grad
+    w.requires_grad_(True)
+    with torch.no_grad():
+        assert not ops.embedding_lookup(w, ids).requires_grad
+    y = ops.embedding_lookup(w * 2.0, ids)  # a table that is no leaf
+    (g,) = torch.autograd.grad(y.sum(), w)
+    want = torch.zeros(20, 8)
+    want[:6] = 2.0
+    assert torch.equal(g.cpu(), want)
+
+
 @pytest.mark.parametrize("n", [200, 6000, 100000])
 def test_on_another_stream(n):
     V, D = 3000, 64
@@ -427,7 +455,8 @@ def test_clip_tells_autograd_and_refuses():
     for call in (
             lambda: ops.global_norm([w]), lambda: ops.clip_by_global_norm_([w], 1.0),
             lambda: ops.global_norm([x.double()]), lambda: ops.global_norm([x, x.cpu()]),
-            lambda: ops.global_norm([z[:, :3]]), lambda: ops.global_norm([x[:1].expand(8)]),
+            lambda: ops.global_norm([z[:, :3]]), lambda: ops.global_norm([z[::2].t()]),
+            lambda: ops.global_norm(z), lambda: ops.global_norm([x[:1].expand(8)]),
             lambda: ops.global_norm([x.to_sparse()]),
             lambda: ops.clip_by_global_norm_([x, x], 1.0),
             lambda: ops.clip_by_global_norm_([x, x[4:]], 1.0),

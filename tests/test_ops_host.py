@@ -135,17 +135,10 @@ def test_python_layer_has_no_cpu_fallback():
             call()
     with pytest.raises(ValueError, match="tensor"):
         ops.global_norm([1.0])
+    with pytest.raises(ValueError, match="list of tensors"):
+        ops.global_norm(w)
     with pytest.raises(ValueError, match="tensor"):
         ops.embedding_lookup(np.zeros((4, 3), np.float32), i)
-
-
-@pytest.mark.parametrize("shape,perm,dense", [
-    ((3, 4, 5), (0, 1, 2), True), ((3, 4, 5), (2, 0, 1), True), ((1, 4, 1), (2, 1, 0), True)])
-def test_dense_in_any_order(shape, perm, dense):
-    assert ops._is_dense(torch.zeros(shape).permute(perm)) is dense
-    assert not ops._is_dense(torch.zeros(6, 4)[:, :3])
-    assert not ops._is_dense(torch.zeros(6, 4)[::2].t())
-    assert not ops._is_dense(torch.zeros(1, 4).expand(6, 4))
 
 
 def test_classifier_on_the_cpu_trains_its_table():
