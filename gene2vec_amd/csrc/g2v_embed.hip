@@ -174,14 +174,48 @@ __device__ __forceinline__ int block_scan(int x, int& all) {
   return before + s - x;
 }
 
-// the place of this lane's token: next[key] plus the lower lanes of that key;
-// next[key] moves on by all of them
-__device__ __forceinline__ int place_keys(uint32_t* next, int key, bool has, int bits) {
+// Where one key is most of the wave (a bucket with a very frequent row) it is
+// cheaper to take whole keys out one by one than to compare bit by bit: taken
+// by the lowest lane left, first once, then while few lanes are left.
+constexpr int kFewLanes = 6;
+
+__device__ __forceinline__ uint64_t peers_skewed(int key, bool has, int bits) {
+  uint64_t left = __ballot(has), mine = 0;
+  bool first = true;
+  while (left && (first || __popcll(left) <= kFewLanes)) {
+    const int k = __builtin_amdgcn_readlane(key, __builtin_ctzll(left));
+    const bool in = has && key == k;
+    const uint64_t same = __ballot(in);
+    mine = in ? same : mine;
+    left &= ~same;
+    first = false;
+  }
+  if (left) {
+    const bool rest = left >> (threadIdx.x & 63) & 1;
+    const uint64_t m = peers(key, rest, bits);
+    mine = rest ? m : mine;
+  }
+  return mine;
+}
+
+// next[key] += the wave's tokens of that key; the most frequent key, often
+// that of the first lane, with one access
+__device__ __forceinline__ void count_keys(uint32_t* next, int key, bool has) {
+  const uint64_t m = __ballot(has);
+  if (!m) return;
+  const int lead = __builtin_ctzll(m), k = __builtin_amdgcn_readlane(key, lead);
+  const uint64_t same = __ballot(has && key == k);
+  if ((int)(threadIdx.x & 63) == lead) atomicAdd(&next[key], (uint32_t)__popcll(same));
+  else if (has && key != k) atomicAdd(&next[key], 1u);
+}
+
+// the place of this lane's token: next[key] plus the lower lanes of that key
+// (m: all of them); next[key] moves on by all of them
+__device__ __forceinline__ int place_keys(uint32_t* next, int key, bool has, uint64_t m) {
   const int lane = threadIdx.x & 63;
-  const uint64_t m = peers(key, has, bits);
   const int lead = has ? __builtin_ctzll(m) : lane;
   int old = 0;
-  if (has && lead == lane) old = (int)atomicAdd(&next[key], __popcll(m));
+  if (has && lead == lane) old = (int)atomicAdd(&next[key], (uint32_t)__popcll(m));
   return __shfl(old, lead) + __popcll(m & ((1ull << lane) - 1));
 }
 
@@ -202,9 +236,7 @@ __device__ __forceinline__ int sort_bucket(int b, int V, int base, const Sorted&
     if (t < rw)
       for (int w = 0; w < kSortWaves; ++w) hist[w * kKeys + t] = 0;
     __syncthreads();
-    tokens([&](int, int k) {
-      if (k >= w0 && k < w0 + rw) atomicAdd(&mine[k - w0], 1u);
-    });
+    tokens([&](int, int k) { count_keys(mine, k - w0, k >= w0 && k < w0 + rw); });
     __syncthreads();
     int c = 0, all;
     if (t < rw)
@@ -225,7 +257,7 @@ __device__ __forceinline__ int sort_bucket(int b, int V, int base, const Sorted&
     tokens([&](int i, int k) {
       const bool has = k >= w0 && k < w0 + rw;
       if (!__ballot(has)) return;
-      const int p = place_keys(mine, k - w0, has, bits);
+      const int p = place_keys(mine, k - w0, has, peers_skewed(k - w0, has, bits));
       if (!has) return;
       s.perm[p] = i;
       if ((p & ((1 << s.log2L) - 1)) == 0) s.at[p >> s.log2L] = k * kBuckets + b;
@@ -354,7 +386,8 @@ __global__ __launch_bounds__(kSortThreads) void k_tile_scatter(
   for_slice(i0, i1, [&](int64_t i) { return row_of(ids, t0 + i, V, pad); },
             [&](int64_t i, int v) {
               if (!__ballot(v >= 0)) return;
-              const int p = place_keys(mine, v & (kBuckets - 1), v >= 0, 8);
+              const int d = v & (kBuckets - 1);
+              const int p = place_keys(mine, d, v >= 0, peers(d, v >= 0, 8));
               if (v >= 0) pairs[p] = make_int2(v, (int)(t0 + i));
             });
 }
