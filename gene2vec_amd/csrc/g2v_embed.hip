@@ -41,12 +41,15 @@ constexpr int vec_of() {
 // all rows are numbered through and dealt out 1024 to a workgroup, so every
 // width fills the lanes and one row is spread over as many threads as it has
 // vectors; kUnits independent id -> row chains per thread cover the latency.
+// The result goes past the caches, which keep the table's rows instead:
+// 262,144 rows of 512 fp32 from 60,000 take 113 us, with ordinary stores 170;
+// 65,536 of 4,096 bf16 from 131,072 129 us (4.9 TB/s), 157 with ordinary ones.
 template <class TW, class TY, class I, int VEC>
 __global__ __launch_bounds__(kThreads) void k_embed_lookup(
     const TW* __restrict__ W, int64_t V, int D, int64_t ld, const I* __restrict__ ids,
     int64_t units, int nv, float scale, TY* __restrict__ out) {
   const int64_t u0 = block_number() * (kThreads * kUnits);
-  const int64_t row0 = u0 / nv;
+  const int64_t row0 = units <= UINT32_MAX ? (uint32_t)u0 / (uint32_t)nv : u0 / nv;
   const uint32_t r0 = (uint32_t)(u0 - row0 * nv) + threadIdx.x;  // < nv + 1024
   const int64_t left = units - u0;
   int64_t id[kUnits], at[kUnits];
@@ -89,30 +92,39 @@ __global__ __launch_bounds__(kThreads) void k_embed_lookup(
 // lists its own in LDS and counts those of lower buckets, which is where its
 // part of the sorted list begins.  One launch, no exchange between workgroups.
 // Beyond that the tokens are split into buckets first (tile counts, then a
-// stable scatter), and every workgroup reads its bucket alone.
+// stable scatter), and every workgroup reads its bucket alone; a bucket of more
+// than kHotTokens, as a very frequent row makes it, is cut into parts that are
+// counted first and then placed by workgroups of their own.
 
 constexpr int kBuckets = 256;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / 64;
-constexpr int kKeys = 768;          // rows a bucket counts at a time (48 KB of LDS)
+constexpr int kKeys = 1024;         // rows a bucket counts at a time (64 KB of LDS)
 constexpr int kListBits = 10;       // tokens a wave lists: 2^10 (4 KB of LDS)
 constexpr int kScanTokens = kSortWaves << kListBits;
 constexpr int64_t kScanRows = (int64_t)kBuckets << (32 - kListBits);  // a list entry's row
 constexpr int kTileTokens = 1024;
 constexpr int kMaxTiles = 256;      // larger calls take larger tiles
+constexpr int kHotTokens = 4096;    // of a bucket for one workgroup; n / 1024 if more
 constexpr int kPer = 2;             // G vectors of a row that one group takes
 constexpr int kJoinBlocks = 512;
 
 struct Sorted {
   int32_t* perm;    // [n] token positions, row by row
-  int32_t* start;   // [V] first place of row v in perm
-  int32_t* count;   // [V]
+  int2* rows;       // first place in perm and tokens of every row, bucket by bucket
   int32_t* at;      // [n / L + 1] row at every L-th place of perm
   int32_t* longs;   // [n / L + 1] rows of more than L tokens, bucket by bucket
   int32_t* nlong;   // [kBuckets] how many of them
   int32_t* lfirst;  // [kBuckets] where the bucket's begin
   int32_t* total;   // tokens that name a row
   int log2L;
+  int per_bucket;   // rows of a bucket: the stride of `rows`
+  // a bucket's workgroup writes one stretch; by row it would write 8 bytes of
+  // every 256th line that other workgroups write too
+  __device__ __forceinline__ int64_t slot(int v) const {
+    return (int64_t)(v % kBuckets) * per_bucket + v / kBuckets;
+  }
+  __device__ __forceinline__ int2 row(int v) const { return rows[slot(v)]; }
 };
 
 // the lanes of the wave whose key equals this lane's, among those that have one
@@ -219,11 +231,16 @@ __device__ __forceinline__ int place_keys(uint32_t* next, int key, bool has, uin
   return __shfl(old, lead) + __popcll(m & ((1ull << lane) - 1));
 }
 
-// Sorts the tokens of bucket b, which begins at place base.  tokens(f) calls
-// f(position, key) for this wave's tokens of the bucket in order, a whole wave
-// at a time; key: the row over kBuckets, -1 for a lane without a token.
+// Sorts tokens of bucket b, which begins at place base.  tokens(f) calls
+// f(position, key) for this wave's tokens in order, a whole wave at a time; key:
+// the row over kBuckets, -1 for a lane without a token.  They are the bucket's
+// tokens, or part `part` of `parts` of them: then counts holds the tokens of
+// every key in every part (kKeys each; only where the bucket has no more rows).
+// The first part writes what is known of the rows.  Returns the bucket's end.
 template <class T>
-__device__ __forceinline__ int sort_bucket(int b, int V, int base, const Sorted& s, T tokens) {
+__device__ __forceinline__ int sort_bucket(int b, int V, int base, const Sorted& s, int part,
+                                           int parts, const int32_t* __restrict__ counts,
+                                           T tokens) {
   __shared__ uint32_t hist[kSortWaves * kKeys];
   __shared__ int nlong;
   const int rows = V > b ? (V - b + kBuckets - 1) / kBuckets : 0;
@@ -238,15 +255,27 @@ __device__ __forceinline__ int sort_bucket(int b, int V, int base, const Sorted&
     __syncthreads();
     tokens([&](int, int k) { count_keys(mine, k - w0, k >= w0 && k < w0 + rw); });
     __syncthreads();
-    int c = 0, all;
-    if (t < rw)
-      for (int w = 0; w < kSortWaves; ++w) c += (int)hist[w * kKeys + t];
-    int at = base + block_scan(c, all);
+    int c = 0, before = 0, all;
     if (t < rw) {
-      const int v = (w0 + t) * kBuckets + b;
-      s.start[v] = at;
-      s.count[v] = c;
-      if (c > 1 << s.log2L) s.longs[first + atomicAdd(&nlong, 1)] = v;
+      if (parts > 1) {
+#pragma unroll 8
+        for (int q = 0; q < parts; ++q) {
+          const int x = counts[q * kKeys + t];
+          c += x;
+          before += q < part ? x : 0;
+        }
+      } else {
+        for (int w = 0; w < kSortWaves; ++w) c += (int)hist[w * kKeys + t];
+      }
+    }
+    const int start = base + block_scan(c, all);
+    if (t < rw) {
+      if (part == 0) {
+        const int v = (w0 + t) * kBuckets + b;
+        s.rows[(int64_t)b * s.per_bucket + w0 + t] = make_int2(start, c);
+        if (c > 1 << s.log2L) s.longs[first + atomicAdd(&nlong, 1)] = v;
+      }
+      int at = start + before;
       for (int w = 0; w < kSortWaves; ++w) {
         const int h = (int)hist[w * kKeys + t];
         hist[w * kKeys + t] = (uint32_t)at;
@@ -265,9 +294,10 @@ __device__ __forceinline__ int sort_bucket(int b, int V, int base, const Sorted&
     base += all;
     __syncthreads();
   }
-  if (t == 0) {
+  if (t == 0 && part == 0) {
     s.nlong[b] = rows ? nlong : 0;
     s.lfirst[b] = first;
+    if (b == kBuckets - 1) *s.total = base;
   }
   return base;
 }
@@ -302,14 +332,13 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scan(const I* __restrict_
             });
   int base;
   (void)block_scan(below, base);
-  const int end = sort_bucket(b, V, base, s, [&](auto f) {
+  sort_bucket(b, V, base, s, 0, 1, nullptr, [&](auto f) {
     for (int j = lane; j - lane < mine_n; j += 64) {
       const bool in = j < mine_n;
       const uint32_t e = in ? mine[j] : 0;
       f((int)i0 + (int)(e & ((1 << kListBits) - 1)), in ? (int)(e >> kListBits) : -1);
     }
   });
-  if (b == kBuckets - 1 && threadIdx.x == 0) *s.total = end;
 }
 
 // tokens of every bucket in every tile
@@ -347,6 +376,7 @@ __global__ __launch_bounds__(kSortThreads) void k_tile_scatter(
   for (int k = threadIdx.x; k < kSortWaves * kBuckets; k += kSortThreads) hist[k] = 0;
   const int d = threadIdx.x % kBuckets, g = threadIdx.x / kBuckets;
   int before = 0, every = 0;
+#pragma unroll 16
   for (int t = g; t < (int)gridDim.x; t += kSortThreads / kBuckets) {
     const int c = counts[t * kBuckets + d];
     every += c;
@@ -392,13 +422,64 @@ __global__ __launch_bounds__(kSortThreads) void k_tile_scatter(
             });
 }
 
+// The parts of the buckets of more than `hot` tokens, numbered through.
+struct Part {
+  int bucket, part, parts, first;  // first: the number of the bucket's part 0
+};
+
+__device__ __forceinline__ bool part_of(const int32_t* __restrict__ bfirst, int hot, int number,
+                                        Part& p) {
+  __shared__ Part found;
+  int c = 0, all;
+  if (threadIdx.x < kBuckets) {
+    const int n = bfirst[threadIdx.x + 1] - bfirst[threadIdx.x];
+    c = n > hot ? (n + hot - 1) / hot : 0;
+  }
+  const int before = block_scan(c, all);
+  if (number >= before && number < before + c)
+    found = {(int)threadIdx.x, number - before, c, before};
+  __syncthreads();
+  if (number >= all) return false;
+  p = found;
+  return true;
+}
+
+__global__ __launch_bounds__(kSortThreads) void k_hot_count(const int2* __restrict__ pairs,
+                                                            const int32_t* __restrict__ bfirst,
+                                                            int hot, int32_t* __restrict__ counts) {
+  __shared__ uint32_t hist[kKeys];
+  Part p;
+  if (!part_of(bfirst, hot, blockIdx.x, p)) return;
+  hist[threadIdx.x] = 0;
+  __syncthreads();
+  const int64_t lo = bfirst[p.bucket] + (int64_t)p.part * hot, end = bfirst[p.bucket + 1];
+  const int64_t len = end - lo < hot ? end - lo : hot;
+  int64_t i0, i1;
+  my_slice(len, i0, i1);
+  for_slice(i0, i1, [&](int64_t i) { return pairs[lo + i].x / kBuckets; },
+            [&](int64_t, int k) { count_keys(hist, k, k >= 0); });
+  __syncthreads();
+  counts[blockIdx.x * kKeys + threadIdx.x] = (int32_t)hist[threadIdx.x];
+}
+
+// the first workgroups: a part of a hot bucket each, as they take longest; the
+// last kBuckets: a bucket that is not hot
 __global__ __launch_bounds__(kSortThreads) void k_sort_bucket(const int2* __restrict__ pairs,
                                                               const int32_t* __restrict__ bfirst,
-                                                              int V, Sorted s) {
-  const int b = blockIdx.x, lo = bfirst[b];
+                                                              int V, int hot,
+                                                              const int32_t* __restrict__ counts,
+                                                              Sorted s) {
+  const int cold = (int)blockIdx.x - ((int)gridDim.x - kBuckets);
+  Part p{cold, 0, 1, 0};
+  if (cold < 0 && !part_of(bfirst, hot, blockIdx.x, p)) return;
+  const int base = bfirst[p.bucket], end = bfirst[p.bucket + 1];
+  if (cold >= 0 && end - base > hot) return;
+  const int64_t lo = base + (p.parts > 1 ? (int64_t)p.part * hot : 0);
+  const int64_t len = end - lo < hot ? end - lo : hot;
   int64_t i0, i1;
-  my_slice(bfirst[b + 1] - lo, i0, i1);
-  const int end = sort_bucket(b, V, lo, s, [&](auto f) {
+  my_slice(len, i0, i1);
+  sort_bucket(p.bucket, V, base, s, p.part, p.parts, counts + (int64_t)p.first * kKeys,
+              [&](auto f) {
     const int lane = threadIdx.x & 63;
     for (int64_t i = i0; i < i1; i += 256) {
       int2 e[4];
@@ -411,7 +492,6 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_bucket(const int2* __rest
       for (int u = 0; u < 4; ++u) f(e[u].y, e[u].x < 0 ? -1 : e[u].x / kBuckets);
     }
   });
-  if (b == kBuckets - 1 && threadIdx.x == 0) *s.total = end;
 }
 
 // acc += the rows perm[p0 .. p1) of dy, in that order, eight loads in flight
@@ -440,9 +520,12 @@ __device__ __forceinline__ void sum_rows(const TY* __restrict__ dy, int64_t ld,
 }
 
 // G lanes per row; the sum of a row of at most L tokens goes to grad, of none
-// zeros.  A group takes kPer times G vectors of a row, so that the many rows
-// without a token are written by few groups that live long enough to pay for
-// reading the count.
+// zeros.  Memory bound by dy's rows and the whole of grad.  A group takes kPer
+// times G vectors of a row, so that the many rows without a token are written by
+// fewer groups that live long enough to pay for reading the count: 16,384 tokens
+// of 131,072 x 4,096 bf16 take 267 us at 1, 205 at 2, 237 at 4; with ordinary
+// stores, not past the caches, 322 at 2.  The kernel alone takes 160 us there,
+// what filling that gradient takes, and 218 where dy comes from memory.
 //
 // A longer run is cut at every L-th of its tokens into pieces, first in the grid
 // as they take longest and G vectors a group; their sums go to part.  Pieces are
@@ -470,7 +553,8 @@ __global__ __launch_bounds__(kThreads) void k_grad_rows(const TY* __restrict__ d
     const int c = (int)(slot >> 1), later = (int)(slot & 1);
     const int64_t q = (int64_t)(c + 1 - later) << s.log2L;
     if (q >= *s.total) return;
-    const int v = s.at[c + 1 - later], p = s.start[v], n = s.count[v];
+    const int2 run = s.row(s.at[c + 1 - later]);
+    const int p = run.x, n = run.y;
     if (n <= L) return;
     int p0 = p;
     if (later) {
@@ -489,9 +573,9 @@ __global__ __launch_bounds__(kThreads) void k_grad_rows(const TY* __restrict__ d
   const int parts = (tiles + kPer - 1) / kPer;
   const int64_t v = parts == 1 ? r : r / parts;
   if (v >= V) return;
-  const int n = s.count[v];
+  const int2 run = s.row((int)v);
+  const int p = run.x, n = run.y;
   if (n > L) return;
-  const int p = n > 0 ? s.start[v] : 0;
   int unit = (int)(r - v * parts) * kPer * G + lane;
   for (int k = 0; k < kPer && unit < nv; ++k, unit += G) {
     const int col = unit * VEC + VEC <= D ? unit * VEC : D - VEC;
@@ -529,9 +613,10 @@ __global__ __launch_bounds__(kSortThreads) void k_grad_join(Sorted s,
     int b = 0;  // the last bucket with before[b] <= j: it holds run j
     for (int d = kBuckets / 2; d; d >>= 1)
       if (before[b + d] <= j) b += d;
-    const int v = s.longs[s.lfirst[b] + j - before[b]], n = s.count[v];
-    const int pieces = (n + (1 << s.log2L) - 1) >> s.log2L;
-    const int64_t c0 = s.start[v] >> s.log2L;
+    const int v = s.longs[s.lfirst[b] + j - before[b]];
+    const int2 run = s.row(v);
+    const int pieces = (run.y + (1 << s.log2L) - 1) >> s.log2L;
+    const int64_t c0 = run.x >> s.log2L;
     float acc[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
@@ -564,7 +649,9 @@ struct Plan {
   int log2L;
   int64_t chunks, slots;  // places of L tokens; pieces (none where no run can be long)
   int64_t tiles, tile;    // 0: every bucket reads all ids
-  int64_t perm, start, count, at, longs, small, part, pairs, counts, bfirst, bytes;
+  int64_t hot, parts;     // tokens of a part, and the most parts there can be
+  int64_t per_bucket;
+  int64_t perm, rows, at, longs, small, part, pairs, counts, bfirst, hcounts, bytes;
 };
 
 Plan plan(int64_t n, int64_t V, int64_t D) {
@@ -580,6 +667,12 @@ Plan plan(int64_t n, int64_t V, int64_t D) {
     p.tile = (n + kMaxTiles - 1) / kMaxTiles;
     p.tile = p.tile < kTileTokens ? kTileTokens : (p.tile + kSortThreads - 1) / kSortThreads * kSortThreads;
     p.tiles = (n + p.tile - 1) / p.tile;
+    // a bucket is cut where its rows fit one window of counts
+    p.hot = n / 1024 > kHotTokens ? n / 1024 : kHotTokens;
+    if (V > (int64_t)kBuckets * kKeys) p.hot = n > 0 ? n : 1;
+    // a hot bucket of m tokens has fewer than m / hot + 1 parts
+    const int64_t most = n / p.hot;
+    p.parts = p.hot < n ? most + (most < kBuckets ? most : kBuckets) : 0;
   }
   const auto take = [&](int64_t count, int64_t size) {
     const int64_t o = p.bytes;
@@ -587,8 +680,8 @@ Plan plan(int64_t n, int64_t V, int64_t D) {
     return o;
   };
   p.perm = take(n, 4);
-  p.start = take(V, 4);
-  p.count = take(V, 4);
+  p.per_bucket = (V + kBuckets - 1) / kBuckets;
+  p.rows = take(p.per_bucket * kBuckets, 8);
   p.at = take(p.chunks + 1, 4);
   p.longs = take(p.chunks + 1, 4);
   p.small = take(2 * kBuckets + 1, 4);
@@ -596,6 +689,7 @@ Plan plan(int64_t n, int64_t V, int64_t D) {
   p.pairs = take(p.tiles ? n : 0, 8);
   p.counts = take(p.tiles * kBuckets, 4);
   p.bfirst = take(p.tiles ? kBuckets + 1 : 0, 4);
+  p.hcounts = take(p.parts * kKeys, 4);
   return p;
 }
 
@@ -697,8 +791,14 @@ int launch_sort(const I* ids, int64_t n, int64_t V, int pad, const Plan& p, cons
     hipLaunchKernelGGL(k_tile_scatter<I>, dim3((unsigned)p.tiles), dim3(kSortThreads), 0, st, ids,
                        n, p.tile, (int)V, pad, counts, bfirst, pairs);
     OP_HIP(hipGetLastError(), "g2v_embed_grad");
-    hipLaunchKernelGGL(k_sort_bucket, dim3(kBuckets), dim3(kSortThreads), 0, st, pairs, bfirst,
-                       (int)V, s);
+    int32_t* hcounts = reinterpret_cast<int32_t*>(ws + p.hcounts);
+    if (p.parts) {
+      hipLaunchKernelGGL(k_hot_count, dim3((unsigned)p.parts), dim3(kSortThreads), 0, st, pairs,
+                         bfirst, (int)p.hot, hcounts);
+      OP_HIP(hipGetLastError(), "g2v_embed_grad");
+    }
+    hipLaunchKernelGGL(k_sort_bucket, dim3((unsigned)(kBuckets + p.parts)), dim3(kSortThreads), 0,
+                       st, pairs, bfirst, (int)V, (int)p.hot, hcounts, s);
   }
   OP_HIP(hipGetLastError(), "g2v_embed_grad");
   return G2V_OK;
@@ -782,8 +882,11 @@ extern "C" int g2v_embed_grad(int device, const void* dy, int dy_type, int64_t d
   char* ws = static_cast<char*>(workspace);
   const auto ints = [&](int64_t o) { return reinterpret_cast<int32_t*>(ws + o); };
   int32_t* small = ints(p.small);
-  const Sorted s{ints(p.perm),  ints(p.start),    ints(p.count),        ints(p.at), ints(p.longs),
-                 small,         small + kBuckets, small + 2 * kBuckets, p.log2L};
+  const Sorted s{ints(p.perm),  reinterpret_cast<int2*>(ws + p.rows),
+                 ints(p.at),    ints(p.longs),
+                 small,         small + kBuckets,
+                 small + 2 * kBuckets, p.log2L,
+                 (int)p.per_bucket};
   float* part = reinterpret_cast<float*>(ws + p.part);
   rc = by_id(id_bytes, [&](auto i) {
     using I = decltype(i);

@@ -45,6 +45,11 @@ def make_ids(kind, V, n, dtype, seed):
         ids = np.full(n, V - 1, np.int64)
     elif kind == "two":
         ids = np.where(rng.random(n) < 0.5, 0, V - 1)
+    elif kind == "skew":  # half the tokens one row, a tenth its bucket's others
+        u = rng.random(n)
+        ids = np.where(u < 0.5, 7 % V, np.where(u < 0.6, rng.integers(0, V, n) // 256 * 256 + 7,
+                                                rng.integers(0, V, n)))
+        ids = ids.clip(0, V - 1)
     elif kind == "sorted":
         ids = np.sort(rng.integers(0, V, n))
     else:
@@ -140,7 +145,10 @@ GRAD = [(1, 1, 1, "uniform"), (1, 5, 200, "same"), (2, 3, 129, "two"), (10, 8, 0
         (256, 64, 64, "absent"), (257, 65, 65, "sorted"), (1000, 301, 1025, "zipf"),
         (24447, 200, 4096, "zipf"), (60000, 12, 5000, "absent"), (131, 1030, 777, "same"),
         (24447, 40, 70001, "zipf"), (300000, 4, 66000, "uniform"), (3, 130, 50000, "two"),
-        (70000, 33, 300007, "zipf"), (512, 16, 262144, "absent"), (700, 4100, 500, "zipf")]
+        (70000, 33, 300007, "zipf"), (512, 16, 262144, "absent"), (700, 4100, 500, "zipf"),
+        (24447, 20, 70001, "skew"), (300000, 8, 70001, "skew"), (256, 16, 20000, "same"),
+        (2, 64, 300000, "two"), (262144, 4, 40000, "skew"), (262145, 4, 40000, "skew"),
+        (5000, 2, 1100000, "skew"), (24447, 16, 16384, "skew"), (24447, 16, 16385, "skew")]
 
 
 @pytest.mark.parametrize("V,D,n,kind", GRAD)
