@@ -9,6 +9,7 @@
 // it in autograd's own thread, and a list of 600 tensors 310 us.
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/Dtype.h>
@@ -74,6 +75,7 @@ const at::Tensor& tensor(py::handle h, const char* name) {
 void on_gpu(const at::Tensor& t, const char* name) {
   if (!t.is_cuda() || t.layout() != at::kStrided)
     refuse(std::string(name) + " must be a dense tensor on the GPU (there is no CPU fallback)");
+  if (t.is_neg()) refuse(std::string(name) + ": a lazily negated view; resolve_neg() it first");
 }
 
 void check_type(at::ScalarType t, const char* name) {
@@ -137,6 +139,7 @@ at::Tensor lookup(const at::Tensor& params, const at::Tensor& ids, int64_t ld, d
 at::Tensor lookup_grad(at::Tensor dy, const at::Tensor& ids, int64_t V, int64_t D, double scale,
                        int64_t pad, at::ScalarType type) {
   const int64_t n = ids.numel();
+  dy = dy.resolve_neg();
   if (dy.dim() != 2) dy = dy.reshape({n, D});
   int64_t ld = n > 1 ? dy.stride(0) : D;
   if ((D > 1 && dy.stride(1) != 1) || ld < D) {  // a transposed or broadcast gradient
@@ -155,6 +158,19 @@ at::Tensor lookup_grad(at::Tensor dy, const at::Tensor& ids, int64_t V, int64_t 
 }
 
 namespace ag = torch::autograd;
+
+// A leaf's gradient is accumulated on the stream that its live graph was built
+// on.  Captured on another stream, the backward pass would leave the capture
+// and end it, or the process: refused here, before anything is recorded.
+void check_capture(const at::Tensor& params) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const std::shared_ptr<ag::Node> node = ag::impl::try_get_grad_accumulator(params);
+  if (!node) return;
+  const auto stream = node->stream();
+  if (stream && stream->id() != c10::hip::getCurrentHIPStream(params.device().index()).id())
+    refuse("params: a graph of this leaf from another stream is still alive (its loss, say); "
+           "drop it before capturing");
+}
 
 class EmbeddingLookup : public ag::Function<EmbeddingLookup> {
  public:
@@ -208,8 +224,10 @@ at::Tensor embedding_lookup(py::handle params_, py::handle ids_, double scale,
   const int64_t pad = padding_of(padding_idx, V);
   py::gil_scoped_release released;
   const at::Tensor ids = given.contiguous();
-  if (params.requires_grad() && at::GradMode::is_enabled())
+  if (params.requires_grad() && at::GradMode::is_enabled()) {
+    check_capture(params);
     return EmbeddingLookup::apply(params, ids, ld, scale, pad, (int64_t)type);
+  }
   return lookup(params, ids, ld, scale, type);
 }
 

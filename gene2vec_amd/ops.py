@@ -18,9 +18,10 @@ so calls on several streams do not share any, and a call captured into a
 the same bits.  Wrong arguments raise ``ValueError`` before anything runs, the
 library's own errors ``_native.G2VError``.
 
-A backward pass is captured best on leaves that no live eager graph holds
-(``del`` the loss of earlier steps, ``grad = None``): torch accumulates into a
-leaf on the stream its eager graph was built on, and that ends a capture.
+A lookup in a table that requires its gradient is captured only while no graph
+of that leaf from another stream lives (``del`` the loss of earlier steps): torch
+accumulates on the stream that graph was built on, which ends a capture, so the
+call raises ``ValueError`` then.
 """
 from __future__ import annotations
 

@@ -139,6 +139,19 @@ def test_lookup_keeps_special_values():
     assert math.copysign(1, y[0, 3]) == -1 and bool((y[1] == 0).all())
 
 
+@pytest.mark.parametrize("t", TYPES)
+def test_subnormal_values_are_kept(t):
+    i = torch.finfo(t)
+    w = torch.tensor([[i.tiny / 2, -i.tiny / 4, i.tiny, i.smallest_normal * i.eps, i.max, i.min,
+                       1.0, 0.0, -i.tiny / 8]] * 3, dtype=F32 if t == F32 else t, device="cuda")
+    ids = torch.tensor([0, 1, 2, 2, 0], device="cuda")
+    assert torch.equal(ops.embedding_lookup(w, ids), w[ids])
+    g = ops.embedding_lookup_grad(w[ids[:3]], ids[:3], 4)  # one token a row: sums of one
+    assert torch.equal(g[:3], w) and not g[3].any()
+    out, _ = ops.clip_by_global_norm([w[:, :4].contiguous()], 1e9)
+    assert torch.equal(out[0], w[:, :4])
+
+
 # ---- the gradient ------------------------------------------------------------------------
 GRAD = [(1, 1, 1, "uniform"), (1, 5, 200, "same"), (2, 3, 129, "two"), (10, 8, 0, "uniform"),
         (24447, 200, 1, "uniform"), (12472, 200, 256, "uniform"), (255, 9, 63, "zipf"),
@@ -201,6 +214,11 @@ def test_grad_strides(n):
     t = ids.t()
     dy = wide.transpose(0, 1)
     check_grad(ops.embedding_lookup_grad(dy, t, V), dy, t, V)
+    neg = torch._neg_view(wide)
+    check_grad(ops.embedding_lookup_grad(neg.clone(), ids, V), -wide, ids, V)
+    for call in (lambda: ops.embedding_lookup_grad(neg, ids, V), lambda: ops.global_norm([neg])):
+        with pytest.raises(ValueError, match="negated"):
+            call()
 
 
 def test_offsets_past_32_bits():
@@ -226,6 +244,21 @@ def test_offsets_past_32_bits():
     g = ops.embedding_lookup_grad(y, many, 8, dtype=F32)
     want = torch.bincount(many.cpu(), minlength=8).float()[:, None].expand(8, D)
     assert torch.equal(g.cpu(), want)  # whole numbers below 2^24: exact in any order
+
+
+def test_more_rows_than_a_list_entry_holds():
+    """over 2^30 rows the tokens are sorted without the packed lists"""
+    V = 2**30 + 300
+    for ids in ([], [V - 1, 3, 2**30 + 7, 3, 255, -1, V]):
+        ids = torch.tensor(ids, dtype=torch.int64, device="cuda")
+        dy = torch.arange(1.0, len(ids) + 1, device="cuda")[:, None].to(BF16)
+        g = ops.embedding_lookup_grad(dy, ids, V)
+        if len(ids):
+            for row, want in ((V - 1, 1), (3, 6), (2**30 + 7, 3), (255, 5)):
+                assert float(g[row]) == want
+                g[row] = 0
+        assert not any(bool(part.any()) for part in g.split(2**28))
+        del g
 
 
 # ---- autograd, streams, graphs -----------------------------------------------------------
@@ -315,6 +348,39 @@ def test_on_another_stream(n):
     torch.cuda.synchronize()
     for g in got:
         assert all(torch.equal(x, y) for x, y in zip(g, want))
+
+
+def test_two_threads_at_once():
+    import threading
+    V, D = 2000, 48
+    table = torch.randn(V, D, device="cuda")
+    work = [(make_ids("zipf", V, n, torch.int64, n).cuda(), torch.randn(n, D, device="cuda"))
+            for n in (300, 20000, 5, 70000)]
+    want = [ops.embedding_lookup_grad(dy, ids, V) for ids, dy in work]
+    norms = [ops.global_norm([dy]) for _, dy in work]
+    torch.cuda.synchronize()
+    got, bad = {}, []
+
+    def go(k):
+        try:
+            ids, dy = work[k]
+            w = table.detach().requires_grad_(True)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    g, = torch.autograd.grad(ops.embedding_lookup(w, ids), w, dy)
+                    out, norm = ops.clip_by_global_norm([g, dy], 1.0)
+                    last = g, ops.global_norm([dy])
+                torch.cuda.current_stream().synchronize()
+            got[k] = last
+        except BaseException as e:  # noqa: BLE001
+            bad.append(e)
+
+    threads = [threading.Thread(target=go, args=(k,)) for k in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad, bad
+    for k in range(4):
+        assert torch.equal(got[k][0], want[k]) and torch.equal(got[k][1], norms[k])
 
 
 @pytest.mark.parametrize("n", [100, 5000, 100000])
@@ -595,3 +661,32 @@ def test_captured_training_step():
         eager = ops.embedding_lookup_grad(c, ids, V, 2.0)
         assert torch.equal(norm, ops.clip_by_global_norm_([eager], 1.0))
         assert torch.equal(grad, eager)
+
+
+def test_capture_beside_a_live_eager_graph_is_refused():
+    w = torch.randn(30, 8, device="cuda", requires_grad=True)
+    ids = torch.arange(10, device="cuda")
+    x = torch.ones(4, device="cuda")
+    live = ops.embedding_lookup(w, ids)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        x += 1
+        with pytest.raises(ValueError, match="alive"):
+            ops.embedding_lookup(w, ids)
+        with torch.no_grad():
+            y = ops.embedding_lookup(w, ids)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(x, torch.full_like(x, 2)) and torch.equal(y, w[:10])
+    live.sum().backward()  # the eager graph is still good
+    assert float(w.grad.sum()) == 80.0
+    del live
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        both = ops.embedding_lookup(w, ids) + ops.embedding_lookup(w, ids)
+        grad, = torch.autograd.grad(both.sum(), w)
+    del both
+    g.replay()
+    torch.cuda.synchronize()
+    assert float(grad.sum()) == 160.0
