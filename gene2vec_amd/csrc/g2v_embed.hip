@@ -27,16 +27,12 @@ __device__ __forceinline__ int64_t block_number() {
 
 constexpr int kUnits = 4;  // vectors a thread of the lookup moves
 
-// The elements of a vector: 16 bytes of the narrower of the two types.  A row
-// of D elements is ceil(D / VEC) vectors; the last one ends with the row and
+// Rows are moved in vectors of VEC elements, 16 bytes of one of the types.  A
+// row of D elements is ceil(D / VEC) vectors; the last one ends with the row and
 // overlaps the one before where VEC does not divide D (the same values are
 // written twice), so that no width needs a scalar tail.  Rows narrower than a
 // vector go element by element.
-template <class A, class B>
-constexpr int vec_of() {
-  return 16 / (sizeof(A) < sizeof(B) ? sizeof(A) : sizeof(B));
-}
-
+//
 // Memory bound: a row read and a row written per token, no reuse.  Vectors of
 // all rows are numbered through and dealt out 1024 to a workgroup, so every
 // width fills the lanes and one row is spread over as many threads as it has
@@ -576,16 +572,23 @@ __global__ __launch_bounds__(kThreads) void k_grad_rows(const TY* __restrict__ d
   const int2 run = s.row((int)v);
   const int p = run.x, n = run.y;
   if (n > L) return;
-  int unit = (int)(r - v * parts) * kPer * G + lane;
+  const int first = (int)(r - v * parts) * kPer * G;
+  if (n == 0) {  // zeros, 16 bytes a lane side by side, whatever VEC is
+    constexpr int Z = VEC * sizeof(TG) > 16 ? 16 / sizeof(TG) : VEC;
+    const float zero[Z] = {};
+    const int end = (first + kPer * G) * VEC < D ? (first + kPer * G) * VEC : D;
+    for (int c = first * VEC + lane * Z; c < end; c += G * Z)
+      g2v::store_vec_nt<TG, Z>(grad + v * D + (c + Z <= D ? c : D - Z), zero);
+    return;
+  }
+  int unit = first + lane;
   for (int k = 0; k < kPer && unit < nv; ++k, unit += G) {
     const int col = unit * VEC + VEC <= D ? unit * VEC : D - VEC;
-    if (n > 0) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-      sum_rows<TY, VEC>(dy + col, ld, s.perm, p, p + n, acc);
+    for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+    sum_rows<TY, VEC>(dy + col, ld, s.perm, p, p + n, acc);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] *= scale;
-    }
+    for (int i = 0; i < VEC; ++i) acc[i] *= scale;
     g2v::store_vec_nt<TG, VEC>(grad + v * D + col, acc);
   }
 }
@@ -750,7 +753,9 @@ int by_width(int64_t D, F f) {
 template <class TY, class TG>
 int launch_rows(const TY* dy, int64_t ld, const Sorted& s, int64_t slots, float* part, int64_t V,
                 int64_t D, float scale, TG* grad, hipStream_t st) {
-  return by_width<vec_of<TY, TG>()>(D, [&](auto vec, auto g) {
+  // 16 bytes of the narrower type: dy's rows are most of what is read
+  constexpr int kVec = 16 / (sizeof(TY) < sizeof(TG) ? sizeof(TY) : sizeof(TG));
+  return by_width<kVec>(D, [&](auto vec, auto g) {
     constexpr int VEC = decltype(vec)::value, G = decltype(g)::value;
     const int64_t nv = (D + VEC - 1) / VEC, tiles = (nv + G - 1) / G;
     const int64_t groups = slots * tiles + V * ((tiles + kPer - 1) / kPer);
@@ -823,7 +828,10 @@ extern "C" int g2v_embed_lookup(int device, const void* table, int table_type, i
         using TW = decltype(w);
         using TY = decltype(y);
         using I = decltype(i);
-        constexpr int VEC = vec_of<TW, TY>();
+        // 16 bytes of the result: stores past the caches have to fill their
+        // lines together (262,147 rows of 512, bf16 to fp32: 93 us, with
+        // twice that a lane 227)
+        constexpr int VEC = 16 / sizeof(TY);
         const int64_t nv = D >= VEC ? (D + VEC - 1) / VEC : D;
         const int64_t blocks = (n * nv + kThreads * kUnits - 1) / (kThreads * kUnits);
         hipLaunchKernelGGL((D >= VEC ? k_embed_lookup<TW, TY, I, VEC> : k_embed_lookup<TW, TY, I, 1>),

@@ -6,8 +6,6 @@
 #include <stdint.h>
 #include <stdio.h>
 
-#include <type_traits>
-
 #include "g2v.h"
 #include "g2v_internal.h"
 
@@ -36,22 +34,39 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[VEC]) {
   __builtin_memcpy(p, t, sizeof t);
 }
 
-typedef uint32_t word4_at2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t word4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+// words of an access past the caches, at the alignment of an element
+template <int ALIGN, int BYTES>
+struct Words;
+#define G2V_WORDS(ALIGN, BYTES)                                                              \
+  template <>                                                                                \
+  struct Words<ALIGN, BYTES> {                                                               \
+    typedef uint32_t type                                                                    \
+        __attribute__((ext_vector_type(BYTES / 4), aligned(ALIGN), may_alias));              \
+  };
+G2V_WORDS(2, 8) G2V_WORDS(2, 16) G2V_WORDS(4, 8) G2V_WORDS(4, 16)
+#undef G2V_WORDS
 
-// the same, past the caches: for results larger than they hold
+// how vectors of N bytes are split: 16 bytes an access, 8 where there are no
+// more; 0: single elements take ordinary accesses
+template <int N>
+constexpr int access_bytes() {
+  return N % 16 == 0 ? 16 : N % 8 == 0 ? 8 : 0;
+}
+
+// the same past the caches, for what is not read again soon
 template <class T, int VEC>
 __device__ __forceinline__ void store_vec_nt(T* p, const float (&x)[VEC]) {
-  if constexpr (sizeof(T) * VEC % 16 == 0) {
-    using word4 = std::conditional_t<sizeof(T) == 2, word4_at2, word4_at4>;
+  constexpr int A = access_bytes<sizeof(T) * VEC>();
+  if constexpr (A != 0) {
+    using W = typename Words<sizeof(T), A>::type;
     T t[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) t[i] = (T)x[i];
-    word4 w[sizeof(T) * VEC / 16];
+    W w[sizeof t / A];
     __builtin_memcpy(w, t, sizeof t);
 #pragma unroll
-    for (unsigned k = 0; k < sizeof(T) * VEC / 16; ++k)
-      __builtin_nontemporal_store(w[k], reinterpret_cast<word4*>(p) + k);
+    for (unsigned k = 0; k < sizeof t / A; ++k)
+      __builtin_nontemporal_store(w[k], reinterpret_cast<W*>(p) + k);
   } else {
     store_vec<T, VEC>(p, x);
   }
@@ -59,13 +74,14 @@ __device__ __forceinline__ void store_vec_nt(T* p, const float (&x)[VEC]) {
 
 template <class T, int VEC>
 __device__ __forceinline__ void load_vec_nt(const T* p, float (&x)[VEC]) {
-  if constexpr (sizeof(T) * VEC % 16 == 0) {
-    using word4 = std::conditional_t<sizeof(T) == 2, word4_at2, word4_at4>;
-    word4 w[sizeof(T) * VEC / 16];
-#pragma unroll
-    for (unsigned k = 0; k < sizeof(T) * VEC / 16; ++k)
-      w[k] = __builtin_nontemporal_load(reinterpret_cast<const word4*>(p) + k);
+  constexpr int A = access_bytes<sizeof(T) * VEC>();
+  if constexpr (A != 0) {
+    using W = typename Words<sizeof(T), A>::type;
     T t[VEC];
+    W w[sizeof t / A];
+#pragma unroll
+    for (unsigned k = 0; k < sizeof t / A; ++k)
+      w[k] = __builtin_nontemporal_load(reinterpret_cast<const W*>(p) + k);
     __builtin_memcpy(t, w, sizeof t);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) x[i] = (float)t[i];
