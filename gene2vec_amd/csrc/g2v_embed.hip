@@ -38,8 +38,8 @@ constexpr int kUnits = 4;  // vectors a thread of the lookup moves
 // width fills the lanes and one row is spread over as many threads as it has
 // vectors; kUnits independent id -> row chains per thread cover the latency.
 // The result goes past the caches, which keep the table's rows instead:
-// 262,144 rows of 512 fp32 from 60,000 take 113 us, with ordinary stores 170;
-// 65,536 of 4,096 bf16 from 131,072 129 us (4.9 TB/s), 157 with ordinary ones.
+// 262,144 rows of 512 fp32 from 60,000 take 114 us, with ordinary stores 174;
+// 65,536 of 4,096 bf16 from 131,072 148 us (4.7 TB/s), 159 with ordinary ones.
 template <class TW, class TY, class I, int VEC>
 __global__ __launch_bounds__(kThreads) void k_embed_lookup(
     const TW* __restrict__ W, int64_t V, int D, int64_t ld, const I* __restrict__ ids,
@@ -86,11 +86,13 @@ __global__ __launch_bounds__(kThreads) void k_embed_lookup(
 //
 // Up to kScanTokens tokens every bucket's workgroup reads all ids itself: it
 // lists its own in LDS and counts those of lower buckets, which is where its
-// part of the sorted list begins.  One launch, no exchange between workgroups.
+// part of the sorted list begins.  One launch, no exchange between workgroups
+// (16,384 tokens: 23 us for the gradient, 30 the other way).
 // Beyond that the tokens are split into buckets first (tile counts, then a
 // stable scatter), and every workgroup reads its bucket alone; a bucket of more
 // than kHotTokens, as a very frequent row makes it, is cut into parts that are
-// counted first and then placed by workgroups of their own.
+// counted first and then placed by workgroups of their own (262,144 tokens of
+// one row: 117 us for the gradient of 24,447 x 200, 245 without).
 
 constexpr int kBuckets = 256;
 constexpr int kSortThreads = 1024;
@@ -99,7 +101,7 @@ constexpr int kKeys = 1024;         // rows a bucket counts at a time (64 KB of 
 constexpr int kListBits = 10;       // tokens a wave lists: 2^10 (4 KB of LDS)
 constexpr int kScanTokens = kSortWaves << kListBits;
 constexpr int64_t kScanRows = (int64_t)kBuckets << (32 - kListBits);  // a list entry's row
-constexpr int kTileTokens = 1024;
+constexpr int kTileTokens = 1024;   // 65,536 tokens: 42 us, 45 with 4096
 constexpr int kMaxTiles = 256;      // larger calls take larger tiles
 constexpr int kHotTokens = 4096;    // of a bucket for one workgroup; n / 1024 if more
 constexpr int kPer = 2;             // G vectors of a row that one group takes
@@ -518,10 +520,11 @@ __device__ __forceinline__ void sum_rows(const TY* __restrict__ dy, int64_t ld,
 // G lanes per row; the sum of a row of at most L tokens goes to grad, of none
 // zeros.  Memory bound by dy's rows and the whole of grad.  A group takes kPer
 // times G vectors of a row, so that the many rows without a token are written by
-// fewer groups that live long enough to pay for reading the count: 16,384 tokens
-// of 131,072 x 4,096 bf16 take 267 us at 1, 205 at 2, 237 at 4; with ordinary
-// stores, not past the caches, 322 at 2.  The kernel alone takes 160 us there,
-// what filling that gradient takes, and 218 where dy comes from memory.
+// fewer groups that live long enough to pay for reading the count: the gradient
+// of 16,384 tokens of 131,072 x 4,096 bf16 takes 272 us at 1, 247 at 2, 257 at 4;
+// with ordinary stores, not past the caches, 268 at 2.  218 of the 247 are this
+// kernel (1.2 GB, 5.5 TB/s; 160 where dy is still in the Infinity Cache, which is
+// what filling a tensor of that size takes).
 //
 // A longer run is cut at every L-th of its tokens into pieces, first in the grid
 // as they take longest and G vectors a group; their sums go to part.  Pieces are
@@ -660,19 +663,20 @@ struct Plan {
 Plan plan(int64_t n, int64_t V, int64_t D) {
   Plan p{};
   // short pieces spread a frequent row over more groups, long ones leave less
-  // to join: 65,536 tokens of 24,447 x 200 take 42 us at 64, 43 at 32, 45 at
-  // 128; 262,147 of 60,000 x 512 155 us at 64, 146 at 128, 145 at 256.  A few
-  // hundred tokens are not cut at all, which saves a launch of three.
+  // to join: the gradient of 65,536 tokens of 24,447 x 200 fp32 takes 42 us at
+  // 64, 42 at 32, 46 at 128; of 262,147 of 60,000 x 512 127 us at 64, 122 at 128,
+  // 119 at 256.  A few hundred tokens are not cut at all, which saves a launch of
+  // three (11 us instead of 12).
   p.log2L = n <= 256 ? 8 : n <= 65536 ? 6 : n <= 262144 ? 7 : 8;
   p.chunks = (n + ((int64_t)1 << p.log2L) - 1) >> p.log2L;
   p.slots = n > (int64_t)1 << p.log2L ? 2 * p.chunks : 0;
-  if (n > kScanTokens || V > kScanRows) {
+  if (n > kScanTokens || (n > 0 && V > kScanRows)) {
     p.tile = (n + kMaxTiles - 1) / kMaxTiles;
-    p.tile = p.tile < kTileTokens ? kTileTokens : (p.tile + kSortThreads - 1) / kSortThreads * kSortThreads;
+    p.tile = (p.tile + kTileTokens - 1) / kTileTokens * kTileTokens;
     p.tiles = (n + p.tile - 1) / p.tile;
     // a bucket is cut where its rows fit one window of counts
     p.hot = n / 1024 > kHotTokens ? n / 1024 : kHotTokens;
-    if (V > (int64_t)kBuckets * kKeys) p.hot = n > 0 ? n : 1;
+    if (V > (int64_t)kBuckets * kKeys) p.hot = n;
     // a hot bucket of m tokens has fewer than m / hot + 1 parts
     const int64_t most = n / p.hot;
     p.parts = p.hot < n ? most + (most < kBuckets ? most : kBuckets) : 0;
@@ -834,8 +838,9 @@ extern "C" int g2v_embed_lookup(int device, const void* table, int table_type, i
         constexpr int VEC = 16 / sizeof(TY);
         const int64_t nv = D >= VEC ? (D + VEC - 1) / VEC : D;
         const int64_t blocks = (n * nv + kThreads * kUnits - 1) / (kThreads * kUnits);
-        hipLaunchKernelGGL((D >= VEC ? k_embed_lookup<TW, TY, I, VEC> : k_embed_lookup<TW, TY, I, 1>),
-                           grid_of(blocks), dim3(kThreads), 0, st,
+        const auto kernel =
+            D >= VEC ? k_embed_lookup<TW, TY, I, VEC> : k_embed_lookup<TW, TY, I, 1>;
+        hipLaunchKernelGGL(kernel, grid_of(blocks), dim3(kThreads), 0, st,
                            static_cast<const TW*>(table), V, (int)D, ld,
                            static_cast<const I*>(ids), n * nv, (int)nv, scale,
                            static_cast<TY*>(out));
@@ -867,13 +872,13 @@ extern "C" int g2v_embed_grad(int device, const void* dy, int dy_type, int64_t d
   if (rc == G2V_OK) rc = check_matrix(what, "dy", dy, dy_type, n, dy_ld, D);
   if (rc == G2V_OK) rc = check_matrix(what, "grad", grad, grad_type, V, D, D);
   if (rc != G2V_OK) return rc;
-  OP_REQUIRE(padding_id >= -1 && padding_id < V, G2V_EINVAL, "%s: padding id %lld outside [-1, %lld)",
-             what, (long long)padding_id, (long long)V);
+  OP_REQUIRE(padding_id >= -1 && padding_id < V, G2V_EINVAL,
+             "%s: padding id %lld outside [-1, %lld)", what, (long long)padding_id, (long long)V);
   int64_t need = 0;
   rc = g2v_embed_grad_workspace(n, V, D, &need);
   if (rc != G2V_OK) return rc;
-  OP_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 16 == 0)),
-             G2V_EINVAL, "%s: a 16-byte aligned workspace of %lld bytes is needed (got %lld)", what,
+  OP_REQUIRE(workspace_bytes >= need && workspace && (uintptr_t)workspace % 16 == 0, G2V_EINVAL,
+             "%s: a 16-byte aligned workspace of %lld bytes is needed (got %lld)", what,
              (long long)need, (long long)workspace_bytes);
   g2v::DeviceScope scope(device);
   OP_HIP(scope.error(), what);

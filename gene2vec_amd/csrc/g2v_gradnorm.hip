@@ -6,9 +6,11 @@
 //
 // The squares are formed and added in fp64: an fp32 sum would overflow from
 // elements of 1.8e19 on and lose the small tensors beside the large ones, and
-// the fp64 rate of gfx950 equals its fp32 rate per lane, far above what the
-// memory delivers.  No atomics: every workgroup writes one partial sum, and
-// they are added in a fixed order, so the same gradients give the same bits.
+// gfx950 adds fp64 far faster than memory delivers the elements.  Memory bound:
+// 10^9 bf16 elements in 48 tensors 338 us (5.9 TB/s), clipping 3 * 10^8 elements
+// of two types in 600 tensors 593 us (1 GB read twice and written).  No atomics:
+// every workgroup writes one partial sum, and they are added in a fixed order,
+// so the same gradients give the same bits.
 //
 // The tensors' addresses travel in the kernel arguments, kTensors a launch: no
 // copy from the host, nothing that a captured graph would have to keep alive.

@@ -539,7 +539,8 @@ def test_clip_tells_autograd_and_refuses():
             lambda: ops.clip_by_global_norm([x], 1.0, out=[]),
             lambda: ops.clip_by_global_norm([x], 1.0, out=[y.to(BF16)]),
             lambda: ops.clip_by_global_norm([z], 1.0, out=[torch.ones(8, 8, device="cuda").t()]),
-            lambda: ops.clip_by_global_norm([x], 0.0), lambda: ops.clip_by_global_norm([x], math.inf)):
+            lambda: ops.clip_by_global_norm([x], 0.0),
+            lambda: ops.clip_by_global_norm([x], math.inf)):
         with pytest.raises(ValueError):
             call()
     assert torch.equal(x, torch.ones(8, device="cuda"))

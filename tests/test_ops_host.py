@@ -69,6 +69,11 @@ def test_workspaces_are_asked_for_and_checked():
     if b.value:
         assert _grad(n=5000, V=1000, D=64, dy_ld=64, workspace_bytes=b.value - 1) == N.G2V_EINVAL
         assert _grad(n=5000, V=1000, D=64, dy_ld=64, workspace=P + 8) == N.G2V_EINVAL
+    for n in (0, 1, 64, 256, 257, 16384, 16385, 65536, 262145, 2**24, 2**31 - 1):
+        for V in (1, 255, 256, 262144, 262145, 2**30, 2**30 + 1, 2**31 - 1):
+            for D in (1, 200, 8193):
+                assert L.g2v_embed_grad_workspace(n, V, D, C.byref(b)) == N.G2V_OK
+                assert 4 * n + 8 * V <= b.value < 16 * n + 17 * V + n * D // 2 + 2**25
     assert L.g2v_embed_grad_workspace(-1, 10, 4, C.byref(b)) != N.G2V_OK
     assert L.g2v_embed_grad_workspace(3, 0, 4, C.byref(b)) == N.G2V_EINVAL
     assert L.g2v_embed_grad_workspace(3, 10, 4, None) == N.G2V_EINVAL
