@@ -1,7 +1,7 @@
 // g2v_embed.hip -- embedding lookup with scaling, and its gradient.
 //
 //   y[i]  = scale * W[ids[i]]                       (zero row: ids[i] not in [0, V))
-//   dW[v] = scale * sum over i with ids[i] == v of dy[i], added in token order
+//   dW[v] = scale * sum over i with ids[i] == v of dy[i]
 //
 // GGIPNN's lookup (src/GGIPNN.py:19-25, tf.nn.embedding_lookup) and, for
 // train_embedding=True there, the gradient of its table.

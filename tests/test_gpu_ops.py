@@ -12,12 +12,14 @@ Bounds, u = 2^-24 (half a step of fp32), h = half a step of the type stored
   clip    factor and product round once, then the store:
           |err| <= (2 u + h)(1 + 2^-20) |x| + t
 """
+import ctypes as C
 import math
 
 import numpy as np
 import pytest
 import torch
 
+from gene2vec_amd import _native as N
 from gene2vec_amd import ggipnn as G
 from gene2vec_amd import ops
 
@@ -691,3 +693,96 @@ def test_capture_beside_a_live_eager_graph_is_refused():
     g.replay()
     torch.cuda.synchronize()
     assert float(grad.sum()) == 160.0
+
+
+# ---- the C entries: exact buffers, any workspace contents --------------------------------
+class Guarded:
+    """nbytes of device memory at an offset of its element size from an aligned
+    address, with sentinel bytes on both sides"""
+
+    def __init__(self, nbytes, shift=0, fill=0x5A):
+        self.whole = torch.full((nbytes + 4096,), fill, dtype=torch.uint8, device="cuda")
+        self.at, self.n, self.fill = 2048 + shift, nbytes, fill
+        self.inside = self.whole[self.at:self.at + nbytes]
+
+    def ptr(self):
+        return self.whole.data_ptr() + self.at
+
+    def check(self):
+        w = self.whole
+        assert bool((w[:self.at] == self.fill).all())
+        assert bool((w[self.at + self.n:] == self.fill).all())
+
+
+CODE = {F32: N.F32, F16: N.F16, BF16: N.BF16}
+
+
+@pytest.mark.parametrize("V,D,n,kind", [
+    (1, 1, 1, "same"), (7, 3, 100, "zipf"), (300, 9, 257, "absent"), (999, 13, 5000, "skew"),
+    (257, 200, 16384, "zipf"), (5000, 31, 16385, "zipf"), (2, 17, 40000, "two"),
+    (24447, 5, 70001, "skew"), (262145, 1, 20000, "skew"), (40, 515, 3000, "same")])
+@pytest.mark.parametrize("t", TYPES)
+def test_c_entries_stay_inside_their_buffers(V, D, n, kind, t):
+    L, st = N.lib(), torch.cuda.current_stream().cuda_stream
+    size = torch.finfo(t).bits // 8
+    w = torch.randn(V, D, device="cuda").to(t)
+    dy = torch.randn(n, D, device="cuda").to(t)
+    ids = make_ids(kind, V, n, torch.int32, V).cuda()
+    out = Guarded(n * D * size, size)
+    N.check(L.g2v_embed_lookup(0, w.data_ptr(), CODE[t], V, D, D, ids.data_ptr(), 4, n, 1.5,
+                               out.ptr(), CODE[t], st))
+    out.check()
+    got = out.inside.clone().view(t).view(n, D)
+    assert torch.equal(got, ops.embedding_lookup(w, ids, 1.5))
+    need = C.c_int64()
+    N.check(L.g2v_embed_grad_workspace(n, V, D, C.byref(need)))
+    want = ops.embedding_lookup_grad(dy, ids, V, 1.5, 0)
+    for fill in (0x00, 0x7F, 0xFF):
+        ws, g = Guarded(need.value, 0, fill), Guarded(V * D * size, size, fill)
+        N.check(L.g2v_embed_grad(0, dy.data_ptr(), CODE[t], D, ids.data_ptr(), 4, n, V, D, 1.5, 0,
+                                 g.ptr(), CODE[t], ws.ptr(), need.value, st))
+        ws.check()
+        g.check()
+        assert torch.equal(g.inside.clone().view(t).view(V, D), want)
+
+
+@pytest.mark.parametrize("sizes", [[1], [5, 8191, 8192, 8193], [17] * 129, [1, 70001, 3] * 100])
+def test_c_norm_and_clip_stay_inside_their_buffers(sizes):
+    L, st = N.lib(), torch.cuda.current_stream().cuda_stream
+    types = [TYPES[k % 3] for k in range(len(sizes))]
+    ts = [torch.randn(s, device="cuda").to(t) for s, t in zip(sizes, types)]
+    n = len(ts)
+    outs = [Guarded(s * t.itemsize, t.itemsize) for s, t in zip(sizes, types)]
+    src = (C.c_void_p * n)(*[t.data_ptr() for t in ts])
+    dst = (C.c_void_p * n)(*[o.ptr() for o in outs])
+    numel, codes = (C.c_int64 * n)(*sizes), (C.c_int32 * n)(*[CODE[t] for t in types])
+    need = C.c_int64()
+    N.check(L.g2v_global_norm_workspace(n, C.byref(need)))
+    want, wn = ops.clip_by_global_norm(ts, 0.25)
+    for fill in (0x00, 0x7F, 0xFF):
+        ws, norm = Guarded(need.value, 0, fill), Guarded(4, 4, fill)
+        N.check(L.g2v_global_norm(0, src, numel, codes, n, norm.ptr(), ws.ptr(), need.value, st))
+        assert torch.equal(norm.inside.clone().view(F32)[0], wn)
+        N.check(L.g2v_clip_global_norm(0, src, dst, numel, codes, n, 0.25, norm.ptr(), ws.ptr(),
+                                       need.value, st))
+        assert torch.equal(norm.inside.clone().view(F32)[0], wn)
+        for g in (ws, norm, *outs):
+            g.check()
+        for o, x in zip(outs, want):
+            assert torch.equal(o.inside.clone().view(x.dtype), x)
+
+
+def test_saved_tensor_hooks_and_checkpoints():
+    from torch.utils.checkpoint import checkpoint
+    w = torch.randn(40, 6, device="cuda", requires_grad=True)
+    ids = torch.randint(0, 40, (50,), device="cuda")
+    c = torch.randn(50, 6, device="cuda")
+    want = ops.embedding_lookup_grad(c, ids, 40)
+    with torch.autograd.graph.save_on_cpu():
+        y = ops.embedding_lookup(w, ids)
+    assert torch.equal(torch.autograd.grad(y, w, c)[0], want)
+    y = checkpoint(lambda a: ops.embedding_lookup(a, ids), w, use_reentrant=False)
+    assert torch.equal(torch.autograd.grad(y, w, c)[0], want)
+    y = ops.embedding_lookup(w, ids)
+    for _ in range(2):  # the graph is kept
+        assert torch.equal(torch.autograd.grad(y, w, c, retain_graph=True)[0], want)
