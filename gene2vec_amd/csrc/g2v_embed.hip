@@ -3,8 +3,8 @@
 //   y[i]  = scale * W[ids[i]]                       (zero row: ids[i] not in [0, V))
 //   dW[v] = scale * sum over i with ids[i] == v of dy[i]
 //
-// GGIPNN's lookup (src/GGIPNN.py:19-25, tf.nn.embedding_lookup) and, for
-// train_embedding=True there, the gradient of its table.
+// GGIPNN's lookup (src/GGIPNN.py:19-25) and, for train_embedding=True there, the
+// gradient of its table.
 #include <type_traits>
 
 #include "g2v_ops.h"

@@ -2,7 +2,7 @@
 //
 //   norm = sqrt(sum over tensors and elements of g^2)
 //   clip: dst = g * (clip / max(norm, clip)); NaN everywhere when the norm is
-//         not finite (tf.clip_by_global_norm's rule: an overflow is not hidden)
+//         not finite (an overflow is not hidden)
 //
 // The squares are formed and added in fp64: an fp32 sum would overflow from
 // elements of 1.8e19 on and lose the small tensors beside the large ones, and

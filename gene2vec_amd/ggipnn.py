@@ -18,8 +18,7 @@ pipeline, architecture, initialisers and optimiser:
   train  Adam(1e-3), batch 128, 1 epoch, softmax cross-entropy, l2 = 0
          (GGIPNN_Classification.py:15-30,123-127,208-221); clip_norm (not in
          the reference): the gradients' global norm is held to it before each
-         step (tf.clip_by_global_norm's rule), on the GPU by
-         ``ops.clip_by_global_norm_``
+         step, on the GPU by ``ops.clip_by_global_norm_``
   score  test AUC of softmax[:, 1] (sklearn roc_auc_score, :238-254)
 
 Randomness (unseeded in the reference) is driven by one ``seed`` here.

@@ -6,9 +6,6 @@
     global_norm            the 2-norm over a list of gradients
     clip_by_global_norm    the list scaled down to a norm; ``_`` at the end: in place
 
-The names are those of the TF1 calls the reference's classifier is written in
-(tf.nn.embedding_lookup, tf.global_norm, tf.clip_by_global_norm).
-
 They run in ``libg2v.so`` on the tensors' own device and on torch's current
 stream there, without synchronising; there is no CPU fallback.  Tensors that
 another stream made are the caller's to wait for, and to ``record_stream``, as

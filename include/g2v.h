@@ -478,7 +478,7 @@ int g2v_cosine_pairs(int device, const float *vectors, int64_t V, int32_t D, con
 /* out[i][d] = scale * table[ids[i]][d] for i < n, d < D, formed in fp32 and
  * rounded once; a zero row where ids[i] is outside [0, V).  table: V rows of
  * D elements every ld elements; out: dense [n][D]; ids: int32 (id_bytes 4) or
- * int64 (8).  tf.nn.embedding_lookup (src/GGIPNN.py:24), absent tokens added. */
+ * int64 (8).  GGIPNN's lookup (src/GGIPNN.py:24), absent tokens added. */
 int g2v_embed_lookup(int device, const void *table, int table_type, int64_t V, int64_t D,
                      int64_t ld, const void *ids, int id_bytes, int64_t n, float scale, void *out,
                      int out_type, void *stream);
@@ -495,17 +495,17 @@ int g2v_embed_grad(int device, const void *dy, int dy_type, int64_t dy_ld, const
                    void *stream);
 
 /* *norm = sqrt(sum of the squares of all elements of the n tensors), squares
- * and sums in fp64 (tf.global_norm).  tensors[t]: numel[t] contiguous elements
- * of types[t]; empty tensors may be NULL. */
+ * and sums in fp64.  tensors[t]: numel[t] contiguous elements of types[t];
+ * empty tensors may be NULL. */
 int g2v_global_norm_workspace(int64_t n, int64_t *bytes);
 int g2v_global_norm(int device, const void *const *tensors, const int64_t *numel,
                     const int32_t *types, int64_t n, float *norm, void *workspace,
                     int64_t workspace_bytes, void *stream);
 
 /* dst[t] = src[t] * (clip_norm / max(norm, clip_norm)), the factor rounded to
- * fp32 and the product once to the type; *norm as above, before clipping
- * (tf.clip_by_global_norm).  A norm that is not finite makes every element
- * NaN.  dst[t] == src[t] clips in place; any other overlap is refused. */
+ * fp32 and the product once to the type; *norm as above, before the
+ * clipping.  A norm that is not finite makes every element NaN.  dst[t] ==
+ * src[t] clips in place; any other overlap is refused. */
 int g2v_clip_global_norm(int device, const void *const *src, void *const *dst,
                          const int64_t *numel, const int32_t *types, int64_t n, double clip_norm,
                          float *norm, void *workspace, int64_t workspace_bytes, void *stream);
