@@ -160,16 +160,17 @@ at::Tensor lookup_grad(at::Tensor dy, const at::Tensor& ids, int64_t V, int64_t 
 namespace ag = torch::autograd;
 
 // A leaf's gradient is accumulated on the stream that its live graph was built
-// on.  Captured on another stream, the backward pass would leave the capture
-// and end it, or the process: refused here, before anything is recorded.
+// on.  Where that is the default stream, which no capture can take in, a captured
+// backward pass would end the capture, or the process: refused here, before
+// anything is recorded.
 void check_capture(const at::Tensor& params) {
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   const std::shared_ptr<ag::Node> node = ag::impl::try_get_grad_accumulator(params);
   if (!node) return;
   const auto stream = node->stream();
-  if (stream && stream->id() != c10::hip::getCurrentHIPStream(params.device().index()).id())
-    refuse("params: a graph of this leaf from another stream is still alive (its loss, say); "
-           "drop it before capturing");
+  if (stream && stream->id() == c10::hip::getDefaultHIPStream(params.device().index()).id())
+    refuse("params: a graph of this leaf from the default stream is still alive (its loss, "
+           "say); drop it before capturing");
 }
 
 class EmbeddingLookup : public ag::Function<EmbeddingLookup> {

@@ -12,13 +12,13 @@ another stream made are the caller's to wait for, and to ``record_stream``, as
 with any torch operator.  Workspaces come from torch's allocator in each call,
 so calls on several streams do not share any, and a call captured into a
 ``torch.cuda.graph`` keeps its own in the graph's pool.  The same inputs give
-the same bits.  Wrong arguments raise ``ValueError`` before anything runs, the
-library's own errors ``_native.G2VError``.
+the same bits.  Tensors and values that do not fit raise ``ValueError``
+before anything runs, the library's own errors ``_native.G2VError``.
 
 A lookup in a table that requires its gradient is captured only while no graph
-of that leaf from another stream lives (``del`` the loss of earlier steps): torch
-accumulates on the stream that graph was built on, which ends a capture, so the
-call raises ``ValueError`` then.
+of that leaf from the default stream lives (``del`` the loss of earlier steps):
+torch accumulates on the stream that graph was built on, and the default stream
+ends a capture, so the call raises ``ValueError`` then.
 """
 from __future__ import annotations
 

@@ -468,8 +468,9 @@ int g2v_cosine_pairs(int device, const float *vectors, int64_t V, int32_t D, con
  * captured into a HIP graph.  The caller's current device is left as it was.
  * Workspaces are the caller's: 16-byte aligned, of at least the size asked
  * for, holding nothing between calls; calls that may run at the same time
- * need one each.  Pointers are aligned to their element type, no more.  The
- * same inputs give the same bits. */
+ * need one each.  Pointers are aligned to their element type, no more.  Outputs
+ * overlap nothing else except where clipping in place is named.  The same
+ * inputs give the same bits. */
 #define G2V_F32 0
 #define G2V_F16 1
 #define G2V_BF16 2

@@ -686,6 +686,12 @@ def test_capture_beside_a_live_eager_graph_is_refused():
     assert float(w.grad.sum()) == 80.0
     del live
     g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):  # a table that is no leaf, computed in the graph
+        part, = torch.autograd.grad(ops.embedding_lookup(w * 2.0, ids).sum(), w)
+    g.replay()
+    torch.cuda.synchronize()
+    assert float(part.sum()) == 160.0
+    g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         both = ops.embedding_lookup(w, ids) + ops.embedding_lookup(w, ids)
         grad, = torch.autograd.grad(both.sum(), w)
@@ -786,3 +792,22 @@ def test_saved_tensor_hooks_and_checkpoints():
     y = ops.embedding_lookup(w, ids)
     for _ in range(2):  # the graph is kept
         assert torch.equal(torch.autograd.grad(y, w, c, retain_graph=True)[0], want)
+
+
+def test_capture_beside_a_live_graph_of_a_side_stream():
+    """a graph of the leaf that lives on a side stream is joined into the capture"""
+    w = torch.randn(30, 8, device="cuda", requires_grad=True)
+    ids = torch.arange(10, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        live = ops.embedding_lookup(w, ids)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        grad, = torch.autograd.grad(ops.embedding_lookup(w, ids, 3.0).sum(), w)
+    for _ in range(2):
+        g.replay()
+        torch.cuda.synchronize()
+        assert float(grad.sum()) == 240.0
+    assert torch.equal(live.detach(), w.detach()[:10])
