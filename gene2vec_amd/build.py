@@ -24,7 +24,8 @@ UNITS = ([("g2v_sgns_atomic.hip", [f"-DG2V_K={k}"], f"g2v_sgns_atomic_k{k}.o") f
                       "g2v_gradnorm.hip", "g2v_host.cpp", "g2v_ingest.cpp", "g2v_export.cpp")])
 SOURCES = sorted({u[0] for u in UNITS})
 HEADERS = [os.path.join(CSRC, "g2v_internal.h"), os.path.join(CSRC, "g2v_device.h"),
-           os.path.join(CSRC, "g2v_ops.h"), os.path.join(ROOT, "include", "g2v.h")]
+           os.path.join(CSRC, "g2v_ops.h"), os.path.join(CSRC, "g2v_counts.h"),
+           os.path.join(ROOT, "include", "g2v.h")]
 ARCH = "gfx950"
 # k_sgns_atomic's store-or-atomics choice per row is a uniform if / else that
 # must stay a diamond for the loop head to wait with vmcnt(#row instructions)

@@ -7,6 +7,7 @@
 // gradient of its table.
 #include <type_traits>
 
+#include "g2v_counts.h"
 #include "g2v_ops.h"
 
 namespace {
@@ -241,7 +242,7 @@ __device__ __forceinline__ int sort_bucket(int b, int V, int base, const Sorted&
                                            T tokens) {
   __shared__ uint32_t hist[kSortWaves * kKeys];
   __shared__ int nlong;
-  const int rows = V > b ? (V - b + kBuckets - 1) / kBuckets : 0;
+  const int rows = g2v::rows_of_bucket(V, b, kBuckets);
   const int first = base >> s.log2L, t = threadIdx.x;
   uint32_t* mine = hist + (t / 64) * kKeys;
   if (t == 0) nlong = 0;
@@ -431,7 +432,7 @@ __device__ __forceinline__ bool part_of(const int32_t* __restrict__ bfirst, int 
   int c = 0, all;
   if (threadIdx.x < kBuckets) {
     const int n = bfirst[threadIdx.x + 1] - bfirst[threadIdx.x];
-    c = n > hot ? (n + hot - 1) / hot : 0;
+    c = n > hot ? g2v::pieces(n, hot) : 0;
   }
   const int before = block_scan(c, all);
   if (number >= before && number < before + c)
@@ -621,7 +622,7 @@ __global__ __launch_bounds__(kSortThreads) void k_grad_join(Sorted s,
       if (before[b + d] <= j) b += d;
     const int v = s.longs[s.lfirst[b] + j - before[b]];
     const int2 run = s.row(v);
-    const int pieces = (run.y + (1 << s.log2L) - 1) >> s.log2L;
+    const int pieces = g2v::pieces_log2(run.y, s.log2L);
     const int64_t c0 = run.x >> s.log2L;
     float acc[VEC];
 #pragma unroll
