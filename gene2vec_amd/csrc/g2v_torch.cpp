@@ -1,27 +1,36 @@
-// g2v_torch.cpp -- the tensor operators of libg2v as Python calls on torch
-// tensors (gene2vec_amd/_g2v_torch.so; the public functions and their
+// g2v_torch.cpp -- the tensor operators of libg2v as torch operators `g2v::...`
+// and Python calls (gene2vec_amd/_g2v_torch.so; the public functions and their
 // documentation are in gene2vec_amd/ops.py).
 //
-// A shell around the C ABI: it checks the arguments, allocates results and
-// workspaces on torch's allocator, finds the current stream and records the
-// lookup for autograd.  It is compiled because small calls are all host time:
-// the same checks in Python cost a training step of 256 tokens 83 us, most of
-// it in autograd's own thread, and a list of 600 tensors 310 us.
+// A shell around the C ABI in three layers: the Python entry takes its arguments
+// apart, the Autograd kernel records the lookup, the CUDA kernel checks the
+// arguments, allocates results and workspaces on torch's allocator and enqueues
+// the work on the current stream.  The layers call each other through torch's
+// dispatcher, so that whatever sits in between (a tracer, a functional
+// transform, a dispatch mode) sees one operator and not the empty tensors that
+// it fills.  It is compiled because small calls are all host time: the same
+// checks in Python cost a training step of 256 tokens 83 us, most of it in
+// autograd's own thread, and a list of 600 tensors 310 us.
 #include <ATen/ATen.h>
+#include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/Dtype.h>
-#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/library.h>
 
 #include <cmath>
 #include <cstdint>
 #include <limits>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 #include <vector>
 
 #include "g2v.h"
@@ -35,7 +44,7 @@ struct NativeError : std::runtime_error {
   NativeError(int c, const std::string& m) : std::runtime_error(m), code(c) {}
 };
 
-[[noreturn]] void refuse(const std::string& m) { throw py::value_error(m); }
+[[noreturn]] void refuse(const std::string& m) { C10_THROW_ERROR(ValueError, m); }
 
 void native(int rc) {
   if (rc == G2V_OK) return;
@@ -101,10 +110,9 @@ at::ScalarType result_type(py::handle dtype, at::ScalarType otherwise) {
   return t;
 }
 
-double scale_of(double scale) {
+void check_scale(double scale) {
   if (!(std::fabs(scale) <= std::numeric_limits<float>::max()))
     refuse("scale must be finite in fp32, not " + std::to_string(scale));
-  return scale;
 }
 
 // a whole number as Python gives it: int, numpy integer, 3.0
@@ -115,17 +123,79 @@ int64_t whole(py::handle h, const char* name) {
   return (int64_t)d;
 }
 
-int64_t padding_of(py::handle h, int64_t V) {
+// -1, and only that, where there is none
+int64_t padding_of(py::handle h) {
   if (h.is_none()) return -1;
   const int64_t pad = whole(h, "padding_idx");
-  if (pad < 0 || pad >= V)
-    refuse("padding_idx " + std::to_string(pad) + " is not in [0, " + std::to_string(V) + ")");
+  if (pad < 0) refuse("padding_idx " + std::to_string(pad) + " is negative");
   return pad;
 }
 
-at::Tensor lookup(const at::Tensor& params, const at::Tensor& ids, int64_t ld, double scale,
-                  at::ScalarType type) {
+void check_padding(int64_t pad, int64_t V) {
+  if (pad < -1 || pad >= V)
+    refuse("padding_idx " + std::to_string(pad) + " is not in [0, " + std::to_string(V) + ")");
+}
+
+// ---- the operators' handles: calls through the dispatcher ------------------------------
+template <class F>
+c10::TypedOperatorHandle<F> op(const char* name, const char* overload = "") {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, overload).typed<F>();
+}
+
+at::Tensor call_lookup(const at::Tensor& params, const at::Tensor& ids, double scale, int64_t pad,
+                       at::ScalarType type) {
+  static const auto h = op<at::Tensor(const at::Tensor&, const at::Tensor&, double, int64_t,
+                                      at::ScalarType)>("g2v::embedding_lookup");
+  return h.call(params, ids, scale, pad, type);
+}
+
+at::Tensor call_lookup_grad(const at::Tensor& dy, const at::Tensor& ids, int64_t V, double scale,
+                            int64_t pad, at::ScalarType type) {
+  static const auto h = op<at::Tensor(const at::Tensor&, const at::Tensor&, int64_t, double,
+                                      int64_t, at::ScalarType)>("g2v::embedding_lookup_grad");
+  return h.call(dy, ids, V, scale, pad, type);
+}
+
+at::Tensor call_norm(at::TensorList t_list) {
+  static const auto h = op<at::Tensor(at::TensorList)>("g2v::global_norm");
+  return h.call(t_list);
+}
+
+using Clipped = std::tuple<std::vector<at::Tensor>, at::Tensor>;
+
+Clipped call_clip(at::TensorList t_list, double clip_norm) {
+  static const auto h = op<Clipped(at::TensorList, double)>("g2v::clip_by_global_norm");
+  return h.call(t_list, clip_norm);
+}
+
+at::Tensor call_clip_out(at::TensorList t_list, double clip_norm, at::TensorList out) {
+  static const auto h =
+      op<at::Tensor(at::TensorList, double, at::TensorList)>("g2v::clip_by_global_norm", "out");
+  return h.call(t_list, clip_norm, out);
+}
+
+at::Tensor call_clip_(at::TensorList t_list, double clip_norm) {
+  static const auto h = op<at::Tensor(at::TensorList, double)>("g2v::clip_by_global_norm_");
+  return h.call(t_list, clip_norm);
+}
+
+// ---- the lookup --------------------------------------------------------------------------
+at::Tensor lookup_cuda(const at::Tensor& params, const at::Tensor& given, double scale,
+                       int64_t pad, at::ScalarType type) {
+  on_gpu(params, "params");
+  if (params.dim() != 2 || params.numel() == 0)
+    refuse("params must be a matrix [V, D], not " + shape_of(params.sizes()));
+  check_type(params.scalar_type(), "params");
+  check_type(type, "dtype");
   const int64_t V = params.size(0), D = params.size(1);
+  if (D > 1 && params.stride(1) != 1)
+    refuse("the elements of a row of params must be contiguous");
+  const int64_t ld = V > 1 ? params.stride(0) : D;
+  if (ld < D) refuse("the rows of params overlap (strides " + shape_of(params.strides()) + ")");
+  check_ids(given, params);
+  check_scale(scale);
+  check_padding(pad, V);
+  const at::Tensor ids = given.contiguous();
   std::vector<int64_t> shape(ids.sizes().begin(), ids.sizes().end());
   shape.push_back(D);
   at::Tensor out = at::empty(shape, params.options().dtype(type));
@@ -136,11 +206,22 @@ at::Tensor lookup(const at::Tensor& params, const at::Tensor& ids, int64_t ld, d
   return out;
 }
 
-at::Tensor lookup_grad(at::Tensor dy, const at::Tensor& ids, int64_t V, int64_t D, double scale,
-                       int64_t pad, at::ScalarType type) {
-  const int64_t n = ids.numel();
-  dy = dy.resolve_neg();
-  if (dy.dim() != 2) dy = dy.reshape({n, D});
+at::Tensor lookup_grad_cuda(const at::Tensor& given, const at::Tensor& tokens, int64_t V,
+                            double scale, int64_t pad, at::ScalarType type) {
+  on_gpu(given, "dy");
+  check_ids(tokens, given);
+  check_type(given.scalar_type(), "dy");
+  check_type(type, "dtype");
+  if (given.dim() != tokens.dim() + 1 ||
+      given.sizes().slice(0, tokens.dim()) != tokens.sizes() || given.size(-1) < 1)
+    refuse("dy " + shape_of(given.sizes()) + " does not hold a row for each of ids " +
+           shape_of(tokens.sizes()));
+  if (V < 1) refuse("vocab_size must be positive, not " + std::to_string(V));
+  check_scale(scale);
+  check_padding(pad, V);
+  const at::Tensor ids = tokens.contiguous();
+  const int64_t n = ids.numel(), D = given.size(-1);
+  at::Tensor dy = given.dim() == 2 ? given : given.reshape({n, D});
   int64_t ld = n > 1 ? dy.stride(0) : D;
   if ((D > 1 && dy.stride(1) != 1) || ld < D) {  // a transposed or broadcast gradient
     dy = dy.contiguous();
@@ -173,63 +254,82 @@ void check_capture(const at::Tensor& params) {
            "say); drop it before capturing");
 }
 
-class EmbeddingLookup : public ag::Function<EmbeddingLookup> {
- public:
-  static at::Tensor forward(ag::AutogradContext* ctx, const at::Tensor& params,
-                            const at::Tensor& ids, int64_t ld, double scale, int64_t pad,
-                            int64_t type) {
-    ctx->save_for_backward({ids});
-    ctx->saved_data["V"] = params.size(0);
-    ctx->saved_data["D"] = params.size(1);
-    ctx->saved_data["scale"] = scale;
-    ctx->saved_data["pad"] = pad;
-    ctx->saved_data["type"] = (int64_t)params.scalar_type();
-    return lookup(params, ids, ld, scale, (at::ScalarType)type);
+struct EmbeddingLookupBackward : public ag::Node {
+  ag::SavedVariable ids;
+  int64_t V = 0, D = 0, pad = -1;
+  double scale = 1.0;
+  at::TensorOptions table;  // type and device of the gradient
+
+  std::string name() const override { return "EmbeddingLookupBackward"; }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    ids.reset_data();
   }
 
-  static ag::variable_list backward(ag::AutogradContext* ctx, ag::variable_list dy) {
-    const bool again = at::GradMode::is_enabled();
+  ag::variable_list apply(ag::variable_list&& dy) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    const at::Tensor tokens = ids.unpack();
+    if (!task_should_compute_output(0)) return {at::Tensor()};
+    // create_graph=True: whoever differentiates the gradient is told
+    const bool again = ag::compute_requires_grad(dy[0]);
     at::Tensor grad;
     {
       at::NoGradGuard no_grad;
-      auto& d = ctx->saved_data;
-      grad = lookup_grad(dy[0].detach(), ctx->get_saved_variables()[0], d["V"].toInt(),
-                         d["D"].toInt(), d["scale"].toDouble(), d["pad"].toInt(),
-                         (at::ScalarType)d["type"].toInt());
+      grad = dy[0].defined() ? call_lookup_grad(dy[0], tokens, V, scale, pad,
+                                                c10::typeMetaToScalarType(table.dtype()))
+                             : at::zeros({V, D}, table);
     }
-    if (again) {  // create_graph=True: whoever differentiates the gradient is told
-      auto error = std::make_shared<ag::DelayedError>(
-          "embedding_lookup is differentiable once, not twice", 1);
-      grad = (*error)({grad.set_requires_grad(true)})[0];
-    }
-    return {grad, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    if (again)
+      ag::set_history(grad, std::make_shared<ag::Error>(
+                                "embedding_lookup is differentiable once, not twice",
+                                ag::collect_next_edges(dy[0])));
+    return {grad};
   }
 };
+
+at::Tensor lookup_autograd(const at::Tensor& params, const at::Tensor& given, double scale,
+                           int64_t pad, at::ScalarType type) {
+  const at::Tensor ids = given.contiguous();
+  std::shared_ptr<EmbeddingLookupBackward> node;
+  if (ag::compute_requires_grad(params)) {
+    check_capture(params);
+    node = std::shared_ptr<EmbeddingLookupBackward>(new EmbeddingLookupBackward, ag::deleteNode);
+    node->set_next_edges(ag::collect_next_edges(params));
+  }
+  at::Tensor out;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = call_lookup(params, ids, scale, pad, type);
+  }
+  if (node) {
+    node->ids = ag::SavedVariable(ids, false);
+    node->V = params.size(0);
+    node->D = params.size(1);
+    node->pad = pad;
+    node->scale = scale;
+    node->table = params.options();
+    ag::set_history(out, node);
+  }
+  return out;
+}
+
+at::Tensor lookup_grad_autograd(const at::Tensor& dy, const at::Tensor& ids, int64_t V,
+                                double scale, int64_t pad, at::ScalarType type) {
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_lookup_grad(dy, ids, V, scale, pad, type);
+}
 
 at::Tensor embedding_lookup(py::handle params_, py::handle ids_, double scale,
                             py::handle padding_idx, py::handle dtype) {
   const at::Tensor& params = tensor(params_, "params");
   on_gpu(params, "params");
-  if (params.dim() != 2 || params.numel() == 0)
-    refuse("params must be a matrix [V, D], not " + shape_of(params.sizes()));
-  check_type(params.scalar_type(), "params");
-  const int64_t V = params.size(0), D = params.size(1);
-  if (D > 1 && params.stride(1) != 1)
-    refuse("the elements of a row of params must be contiguous");
-  const int64_t ld = V > 1 ? params.stride(0) : D;
-  if (ld < D) refuse("the rows of params overlap (strides " + shape_of(params.strides()) + ")");
-  const at::Tensor& given = tensor(ids_, "ids");
-  check_ids(given, params);
+  const at::Tensor& ids = tensor(ids_, "ids");
+  on_gpu(ids, "ids");
   const at::ScalarType type = result_type(dtype, params.scalar_type());
-  scale_of(scale);
-  const int64_t pad = padding_of(padding_idx, V);
+  const int64_t pad = padding_of(padding_idx);
   py::gil_scoped_release released;
-  const at::Tensor ids = given.contiguous();
-  if (params.requires_grad() && at::GradMode::is_enabled()) {
-    check_capture(params);
-    return EmbeddingLookup::apply(params, ids, ld, scale, pad, (int64_t)type);
-  }
-  return lookup(params, ids, ld, scale, type);
+  return call_lookup(params, ids, scale, pad, type);
 }
 
 at::Tensor embedding_lookup_grad(py::handle dy_, py::handle ids_, py::handle vocab_size,
@@ -237,33 +337,150 @@ at::Tensor embedding_lookup_grad(py::handle dy_, py::handle ids_, py::handle voc
   const at::Tensor& dy = tensor(dy_, "dy");
   on_gpu(dy, "dy");
   const at::Tensor& ids = tensor(ids_, "ids");
-  check_ids(ids, dy);
-  check_type(dy.scalar_type(), "dy");
-  if (dy.dim() != ids.dim() + 1 || dy.sizes().slice(0, ids.dim()) != ids.sizes() ||
-      dy.size(-1) < 1)
-    refuse("dy " + shape_of(dy.sizes()) + " does not hold a row for each of ids " +
-           shape_of(ids.sizes()));
-  const int64_t V = whole(vocab_size, "vocab_size");
-  if (V < 1) refuse("vocab_size must be positive, not " + std::to_string(V));
+  on_gpu(ids, "ids");
   const at::ScalarType type = result_type(dtype, dy.scalar_type());
-  scale_of(scale);
-  const int64_t pad = padding_of(padding_idx, V);
+  const int64_t V = whole(vocab_size, "vocab_size"), pad = padding_of(padding_idx);
   py::gil_scoped_release released;
-  at::NoGradGuard no_grad;
-  return lookup_grad(dy.detach(), ids.contiguous(), V, dy.size(-1), scale, pad, type);
+  return call_lookup_grad(dy, ids, V, scale, pad, type);
 }
 
+// ---- norm and clipping -------------------------------------------------------------------
 // its elements fill one stretch of memory, each once, in whatever order
 bool is_dense(const at::Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }
 
-// a list of tensors as the C entries take it, without its None entries
+// a list of tensors as the C entries take it
 struct List {
-  std::vector<at::Tensor> tensors;
   std::vector<const void*> src;
   std::vector<int64_t> numel;
   std::vector<int32_t> types;
-  size_t size() const { return tensors.size(); }
+  at::Tensor norm, ws;
+  int device = 0;
+
+  List(at::TensorList tensors, const char* what) {
+    const size_t n = tensors.size();
+    if (!n) refuse(std::string(what) + ": the list holds no tensor");
+    src.reserve(n);
+    numel.reserve(n);
+    types.reserve(n);
+    for (const at::Tensor& t : tensors) {
+      on_gpu(t, what);
+      if (t.device() != tensors[0].device())
+        refuse(std::string(what) + ": tensors on " + tensors[0].device().str() + " and " +
+               t.device().str());
+      const int type = type_code(t.scalar_type());
+      if (type < 0)
+        refuse(std::string(what) + ": tensors must be float32, float16 or bfloat16, not " +
+               name_of(t.scalar_type()));
+      if (!is_dense(t))
+        refuse(std::string(what) + ": the elements of a tensor must be dense in memory (shape " +
+               shape_of(t.sizes()) + ", strides " + shape_of(t.strides()) + ")");
+      src.push_back(t.const_data_ptr());
+      numel.push_back(t.numel());
+      types.push_back(type);
+    }
+    int64_t bytes = 0;
+    native(g2v_global_norm_workspace((int64_t)n, &bytes));
+    norm = at::empty({}, tensors[0].options().dtype(at::kFloat));
+    ws = at::empty({bytes}, tensors[0].options().dtype(at::kByte));
+    device = device_index(norm);
+  }
 };
+
+at::Tensor norm_cuda(at::TensorList t_list) {
+  const List l(t_list, "global_norm");
+  native(g2v_global_norm(l.device, l.src.data(), l.numel.data(), l.types.data(),
+                         (int64_t)l.src.size(), l.norm.mutable_data_ptr<float>(),
+                         l.ws.mutable_data_ptr(), l.ws.numel(), stream_of(l.norm)));
+  return l.norm;
+}
+
+// t_list into outs, of the same shapes, types and strides; outs may be t_list
+at::Tensor clip_into(at::TensorList t_list, at::TensorList outs, double clip_norm,
+                     const char* what) {
+  if (!(clip_norm > 0.0 && clip_norm < std::numeric_limits<double>::infinity()))
+    refuse(std::string(what) + ": clip_norm must be positive and finite, not " +
+           std::to_string(clip_norm));
+  const List l(t_list, what);
+  std::vector<void*> dst;
+  dst.reserve(outs.size());
+  for (const at::Tensor& o : outs) {
+    if (o.is_inference() && !c10::InferenceMode::is_enabled())
+      refuse(std::string(what) + ": an inference tensor is written in inference mode only");
+    dst.push_back(o.mutable_data_ptr());
+  }
+  const int rc = g2v_clip_global_norm(
+      l.device, l.src.data(), dst.data(), l.numel.data(), l.types.data(), (int64_t)l.src.size(),
+      clip_norm, l.norm.mutable_data_ptr<float>(), l.ws.mutable_data_ptr(), l.ws.numel(),
+      stream_of(l.norm));
+  if (rc == G2V_EINVAL) refuse(g2v_last_error());  // tensors that overlap
+  native(rc);
+  for (const at::Tensor& o : outs)  // autograd learns that they changed
+    if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
+  return l.norm;
+}
+
+Clipped clip_cuda(at::TensorList t_list, double clip_norm) {
+  std::vector<at::Tensor> outs;
+  outs.reserve(t_list.size());
+  for (const at::Tensor& t : t_list) outs.push_back(at::empty_like(t));
+  at::Tensor norm = clip_into(t_list, outs, clip_norm, "clip_by_global_norm");
+  return {std::move(outs), std::move(norm)};
+}
+
+at::Tensor clip_out_cuda(at::TensorList t_list, double clip_norm, at::TensorList out) {
+  const char* what = "clip_by_global_norm";
+  if (out.size() != t_list.size())
+    refuse(std::string(what) + ": " + std::to_string(out.size()) + " outputs for " +
+           std::to_string(t_list.size()) + " tensors");
+  for (size_t i = 0; i < out.size(); ++i) {
+    const at::Tensor &o = out[i], &t = t_list[i];
+    on_gpu(o, "clip_by_global_norm: out");
+    if (o.sizes() != t.sizes() || o.scalar_type() != t.scalar_type() ||
+        o.device() != t.device() ||
+        !((o.is_contiguous() && t.is_contiguous()) || o.strides() == t.strides()))
+      refuse(std::string(what) +
+             ": an output differs from its tensor in shape, type, strides or device");
+  }
+  return clip_into(t_list, out, clip_norm, what);
+}
+
+at::Tensor clip_inplace_cuda(at::TensorList t_list, double clip_norm) {
+  return clip_into(t_list, t_list, clip_norm, "clip_by_global_norm_");
+}
+
+// none of these has a derivative
+void no_derivative(at::TensorList tensors, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor& t : tensors)
+    if (t.requires_grad())
+      refuse(std::string(what) +
+             " is not differentiable: pass gradients, or call it under no_grad()");
+}
+
+at::Tensor norm_autograd(at::TensorList t_list) {
+  no_derivative(t_list, "global_norm");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_norm(t_list);
+}
+
+Clipped clip_autograd(at::TensorList t_list, double clip_norm) {
+  no_derivative(t_list, "clip_by_global_norm");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_clip(t_list, clip_norm);
+}
+
+at::Tensor clip_out_autograd(at::TensorList t_list, double clip_norm, at::TensorList out) {
+  no_derivative(t_list, "clip_by_global_norm");
+  no_derivative(out, "clip_by_global_norm: out");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_clip_out(t_list, clip_norm, out);
+}
+
+at::Tensor clip_inplace_autograd(at::TensorList t_list, double clip_norm) {
+  no_derivative(t_list, "clip_by_global_norm_");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_clip_(t_list, clip_norm);
+}
 
 std::vector<py::object> items_of(py::handle seq, const char* what) {
   std::vector<py::object> v;
@@ -272,137 +489,69 @@ std::vector<py::object> items_of(py::handle seq, const char* what) {
   return v;
 }
 
-List list_of(const std::vector<py::object>& items, const char* what) {
-  List l;
-  const size_t n = items.size();
-  l.tensors.reserve(n);
-  l.src.reserve(n);
-  l.numel.reserve(n);
-  l.types.reserve(n);
-  const bool grad = at::GradMode::is_enabled();
+// the tensors among them, without the None entries
+std::vector<at::Tensor> tensors_of(const std::vector<py::object>& items, const char* what) {
+  std::vector<at::Tensor> v;
+  v.reserve(items.size());
   for (const py::object& o : items) {
     if (o.is_none()) continue;
     if (!THPVariable_Check(o.ptr()))
       refuse(std::string(what) + ": the list must hold tensors, not " + Py_TYPE(o.ptr())->tp_name);
-    const at::Tensor& t = THPVariable_Unpack(o.ptr());
-    on_gpu(t, what);
-    if (l.size() && t.device() != l.tensors[0].device())
-      refuse(std::string(what) + ": tensors on " + l.tensors[0].device().str() + " and " +
-             t.device().str());
-    const int type = type_code(t.scalar_type());
-    if (type < 0)
-      refuse(std::string(what) + ": tensors must be float32, float16 or bfloat16, not " +
-             name_of(t.scalar_type()));
-    if (grad && t.requires_grad())
-      refuse(std::string(what) +
-             " is not differentiable: pass gradients, or call it under no_grad()");
-    if (!is_dense(t))
-      refuse(std::string(what) + ": the elements of a tensor must be dense in memory (shape " +
-             shape_of(t.sizes()) + ", strides " + shape_of(t.strides()) + ")");
-    l.tensors.push_back(t);
-    l.src.push_back(t.const_data_ptr());
-    l.numel.push_back(t.numel());
-    l.types.push_back(type);
+    v.push_back(THPVariable_Unpack(o.ptr()));
+    on_gpu(v.back(), what);
   }
-  if (!l.size()) refuse(std::string(what) + ": the list holds no tensor");
-  return l;
-}
-
-at::Tensor norm_workspace(const List& l) {
-  int64_t bytes = 0;
-  native(g2v_global_norm_workspace((int64_t)l.size(), &bytes));
-  return at::empty({bytes}, l.tensors[0].options().dtype(at::kByte));
+  if (v.empty()) refuse(std::string(what) + ": the list holds no tensor");
+  return v;
 }
 
 at::Tensor global_norm(py::handle t_list) {
-  const std::vector<py::object> items = items_of(t_list, "global_norm");
-  const List l = list_of(items, "global_norm");
+  const std::vector<at::Tensor> tensors = tensors_of(items_of(t_list, "global_norm"),
+                                                     "global_norm");
   py::gil_scoped_release released;
-  at::Tensor norm = at::empty({}, l.tensors[0].options().dtype(at::kFloat));
-  at::Tensor ws = norm_workspace(l);
-  native(g2v_global_norm(device_index(norm), l.src.data(), l.numel.data(), l.types.data(),
-                         (int64_t)l.size(), norm.mutable_data_ptr<float>(), ws.mutable_data_ptr(),
-                         ws.numel(), stream_of(norm)));
-  return norm;
+  return call_norm(tensors);
 }
 
-at::Tensor clip(const List& l, const std::vector<at::Tensor>& outs, double clip_norm,
-                const char* what) {
-  if (!(clip_norm > 0.0 && clip_norm < std::numeric_limits<double>::infinity()))
-    refuse(std::string(what) + ": clip_norm must be positive and finite, not " +
-           std::to_string(clip_norm));
-  std::vector<void*> dst;
-  dst.reserve(outs.size());
-  for (const at::Tensor& o : outs) {
-    if (o.is_inference() && !c10::InferenceMode::is_enabled())
-      refuse(std::string(what) + ": an inference tensor is written in inference mode only");
-    dst.push_back(o.mutable_data_ptr());
-  }
-  at::Tensor norm = at::empty({}, l.tensors[0].options().dtype(at::kFloat));
-  at::Tensor ws = norm_workspace(l);
-  const int rc = g2v_clip_global_norm(
-      device_index(norm), l.src.data(), dst.data(), l.numel.data(), l.types.data(),
-      (int64_t)l.size(), clip_norm, norm.mutable_data_ptr<float>(), ws.mutable_data_ptr(),
-      ws.numel(), stream_of(norm));
-  if (rc == G2V_EINVAL) refuse(g2v_last_error());  // tensors that overlap
-  native(rc);
-  for (const at::Tensor& o : outs)  // autograd learns that they changed
-    if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
-  return norm;
-}
+py::object wrap(at::Tensor t);
 
 py::tuple clip_by_global_norm(py::handle t_list, double clip_norm, py::handle out) {
   const char* what = "clip_by_global_norm";
   const std::vector<py::object> items = items_of(t_list, what);
-  const List l = list_of(items, what);
-  std::vector<at::Tensor> outs;
-  outs.reserve(l.size());
+  const std::vector<at::Tensor> tensors = tensors_of(items, what);
   py::list result;
+  at::Tensor norm;
   if (out.is_none()) {
-    for (const at::Tensor& t : l.tensors) outs.push_back(at::empty_like(t));
-    size_t k = 0;
-    for (const py::object& o : items) {
-      if (o.is_none()) result.append(py::none());
-      else result.append(py::reinterpret_steal<py::object>(THPVariable_Wrap(outs[k++])));
+    std::vector<at::Tensor> outs;
+    {
+      py::gil_scoped_release released;
+      std::tie(outs, norm) = call_clip(tensors, clip_norm);
     }
+    size_t k = 0;
+    for (const py::object& o : items) result.append(o.is_none() ? py::none() : wrap(outs[k++]));
   } else {
     const std::vector<py::object> given = items_of(out, what);
     if (given.size() != items.size())
       refuse(std::string(what) + ": " + std::to_string(given.size()) + " outputs for " +
              std::to_string(items.size()) + " tensors");
-    const bool grad = at::GradMode::is_enabled();
+    std::vector<at::Tensor> outs;
+    outs.reserve(tensors.size());
     for (size_t i = 0; i < items.size(); ++i) {
-      if (items[i].is_none()) {
-        result.append(py::none());
-        continue;
+      if (!items[i].is_none()) {
+        outs.push_back(tensor(given[i], "clip_by_global_norm: out"));
+        on_gpu(outs.back(), "clip_by_global_norm: out");
       }
-      const at::Tensor& t = l.tensors[outs.size()];
-      const at::Tensor& o = tensor(given[i], "clip_by_global_norm: out");
-      on_gpu(o, "clip_by_global_norm: out");
-      if (o.sizes() != t.sizes() || o.scalar_type() != t.scalar_type() ||
-          o.device() != t.device() ||
-          !((o.is_contiguous() && t.is_contiguous()) || o.strides() == t.strides()))
-        refuse(std::string(what) +
-               ": an output differs from its tensor in shape, type, strides or device");
-      if (grad && o.requires_grad())
-        refuse(std::string(what) + ": an output requires a gradient");
-      outs.push_back(o);
-      result.append(given[i]);
+      result.append(items[i].is_none() ? py::none() : given[i]);
     }
-  }
-  at::Tensor norm;
-  {
     py::gil_scoped_release released;
-    norm = clip(l, outs, clip_norm, what);
+    norm = call_clip_out(tensors, clip_norm, outs);
   }
-  return py::make_tuple(result, py::reinterpret_steal<py::object>(THPVariable_Wrap(norm)));
+  return py::make_tuple(result, wrap(norm));
 }
 
 at::Tensor clip_by_global_norm_(py::handle t_list, double clip_norm) {
-  const std::vector<py::object> items = items_of(t_list, "clip_by_global_norm_");
-  const List l = list_of(items, "clip_by_global_norm_");
+  const char* what = "clip_by_global_norm_";
+  const std::vector<at::Tensor> tensors = tensors_of(items_of(t_list, what), what);
   py::gil_scoped_release released;
-  return clip(l, l.tensors, clip_norm, "clip_by_global_norm_");
+  return call_clip_(tensors, clip_norm);
 }
 
 py::object wrap(at::Tensor t) {
@@ -411,14 +560,46 @@ py::object wrap(at::Tensor t) {
 
 }  // namespace
 
+TORCH_LIBRARY(g2v, m) {
+  m.def("embedding_lookup(Tensor params, Tensor ids, float scale, int padding_idx, "
+        "ScalarType dtype) -> Tensor");
+  m.def("embedding_lookup_grad(Tensor dy, Tensor ids, int vocab_size, float scale, "
+        "int padding_idx, ScalarType dtype) -> Tensor");
+  m.def("global_norm(Tensor[] t_list) -> Tensor");
+  m.def("clip_by_global_norm(Tensor[] t_list, float clip_norm) -> (Tensor[], Tensor)");
+  m.def("clip_by_global_norm.out(Tensor[] t_list, float clip_norm, *, Tensor(a!)[] out) -> Tensor");
+  m.def("clip_by_global_norm_(Tensor(a!)[] t_list, float clip_norm) -> Tensor");
+}
+
+TORCH_LIBRARY_IMPL(g2v, CUDA, m) {
+  m.impl("embedding_lookup", &lookup_cuda);
+  m.impl("embedding_lookup_grad", &lookup_grad_cuda);
+  m.impl("global_norm", &norm_cuda);
+  m.impl("clip_by_global_norm", &clip_cuda);
+  m.impl("clip_by_global_norm.out", &clip_out_cuda);
+  m.impl("clip_by_global_norm_", &clip_inplace_cuda);
+}
+
+TORCH_LIBRARY_IMPL(g2v, Autograd, m) {
+  m.impl("embedding_lookup", &lookup_autograd);
+  m.impl("embedding_lookup_grad", &lookup_grad_autograd);
+  m.impl("global_norm", &norm_autograd);
+  m.impl("clip_by_global_norm", &clip_autograd);
+  m.impl("clip_by_global_norm.out", &clip_out_autograd);
+  m.impl("clip_by_global_norm_", &clip_inplace_autograd);
+}
+
 PYBIND11_MODULE(_g2v_torch, m) {
-  // RuntimeError's subclass of the ctypes layer, with the code
+  // refusals as ValueError; the library's errors as the ctypes layer's
+  // subclass of RuntimeError, with the code
   py::register_local_exception_translator([](std::exception_ptr p) {
     try {
       if (p) std::rethrow_exception(p);
     } catch (const NativeError& e) {
       py::object type = py::module_::import("gene2vec_amd._native").attr("G2VError");
       PyErr_SetObject(type.ptr(), type(e.code, std::string(e.what())).ptr());
+    } catch (const c10::ValueError& e) {
+      PyErr_SetString(PyExc_ValueError, e.what_without_backtrace());
     }
   });
   m.def("abi_version", &g2v_abi_version);
