@@ -271,19 +271,11 @@ struct EmbeddingLookupBackward : public ag::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     const at::Tensor tokens = ids.unpack();
     if (!task_should_compute_output(0)) return {at::Tensor()};
-    // create_graph=True: whoever differentiates the gradient is told
-    const bool again = ag::compute_requires_grad(dy[0]);
-    at::Tensor grad;
-    {
-      at::NoGradGuard no_grad;
-      grad = dy[0].defined() ? call_lookup_grad(dy[0], tokens, V, scale, pad,
-                                                c10::typeMetaToScalarType(table.dtype()))
-                             : at::zeros({V, D}, table);
-    }
-    if (again)
-      ag::set_history(grad, std::make_shared<ag::Error>(
-                                "embedding_lookup is differentiable once, not twice",
-                                ag::collect_next_edges(dy[0])));
+    // in the grad mode of the pass (create_graph=True: recorded)
+    const at::Tensor grad =
+        dy[0].defined() ? call_lookup_grad(dy[0], tokens, V, scale, pad,
+                                           c10::typeMetaToScalarType(table.dtype()))
+                        : at::zeros({V, D}, table);
     return {grad};
   }
 };
@@ -311,13 +303,27 @@ at::Tensor lookup_autograd(const at::Tensor& params, const at::Tensor& given, do
     node->table = params.options();
     ag::set_history(out, node);
   }
+  const at::Tensor& tangent = params._fw_grad(0);  // linear in params
+  if (tangent.defined())
+    out._set_fw_grad(call_lookup(tangent, ids, scale, pad, type), 0, false);
   return out;
 }
 
 at::Tensor lookup_grad_autograd(const at::Tensor& dy, const at::Tensor& ids, int64_t V,
                                 double scale, int64_t pad, at::ScalarType type) {
-  at::AutoDispatchBelowADInplaceOrView below;
-  return call_lookup_grad(dy, ids, V, scale, pad, type);
+  at::Tensor grad;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    grad = call_lookup_grad(dy, ids, V, scale, pad, type);
+  }
+  if (ag::compute_requires_grad(dy))  // whoever differentiates the gradient is told
+    ag::set_history(grad, std::make_shared<ag::Error>(
+                              "embedding_lookup is differentiable once, not twice",
+                              ag::collect_next_edges(dy)));
+  const at::Tensor& tangent = dy._fw_grad(0);  // linear in dy
+  if (tangent.defined())
+    grad._set_fw_grad(call_lookup_grad(tangent, ids, V, scale, pad, type), 0, false);
+  return grad;
 }
 
 at::Tensor embedding_lookup(py::handle params_, py::handle ids_, double scale,
@@ -448,13 +454,16 @@ at::Tensor clip_inplace_cuda(at::TensorList t_list, double clip_norm) {
   return clip_into(t_list, t_list, clip_norm, "clip_by_global_norm_");
 }
 
-// none of these has a derivative
+// none of these has a derivative, backward or forward
 void no_derivative(at::TensorList tensors, const char* what) {
-  if (!at::GradMode::is_enabled()) return;
-  for (const at::Tensor& t : tensors)
-    if (t.requires_grad())
+  const bool grad = at::GradMode::is_enabled();
+  for (const at::Tensor& t : tensors) {
+    if (grad && t.requires_grad())
       refuse(std::string(what) +
              " is not differentiable: pass gradients, or call it under no_grad()");
+    if (t._fw_grad(0).defined())
+      refuse(std::string(what) + " is not differentiable: a tensor has a forward-mode tangent");
+  }
 }
 
 at::Tensor norm_autograd(at::TensorList t_list) {

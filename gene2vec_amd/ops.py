@@ -49,9 +49,9 @@ def embedding_lookup(params, ids, scale=1.0, padding_idx=None, dtype=None):
     padding_idx  a row that gets no gradient (it is looked up like the others)
     dtype        of the result; None: that of params.  One rounding from fp32
 
-    Differentiable in params, once; the gradient is dense [V, D] in the type
-    of params (``embedding_lookup_grad``).  ids that are not contiguous are
-    copied.
+    Differentiable in params, once, and in forward mode; the gradient is dense
+    [V, D] in the type of params (``embedding_lookup_grad``).  ids that are not
+    contiguous are copied.
     """
     return _x.embedding_lookup(params, ids, scale, padding_idx, dtype)
 
@@ -73,7 +73,8 @@ def global_norm(t_list):
 
     Tensors: float32, float16 or bfloat16, mixed as they come, of one device,
     dense in memory in any order of dimensions.  Squares and sums are fp64, so
-    only a norm beyond fp32 itself overflows.  Not differentiable.
+    only a norm beyond fp32 itself overflows.  Not differentiable: a tensor that
+    requires a gradient (in grad mode) or has a forward-mode tangent is refused.
     """
     return _x.global_norm(t_list)
 

@@ -115,3 +115,103 @@ def test_refusals_of_the_registered_operators():
                  lambda: g.clip_by_global_norm.out([w], 1.0, out=[])):
         with pytest.raises((ValueError, NotImplementedError)):
             call()
+
+
+# ---- forward-mode derivatives and functional transforms ----------------------------------
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode(requires_grad):
+    """the lookup is linear in its table, its gradient in dy: the tangent of the
+    result is the operator of the tangent"""
+    import torch.autograd.forward_ad as fwd
+    w, ids, dy = inputs(7)
+    tw, tdy = inputs(8)[::2]
+    want = ops.embedding_lookup(tw, ids, 0.5), ops.embedding_lookup_grad(tdy, ids, V, 0.5, 3)
+    w.requires_grad_(requires_grad)
+    with fwd.dual_level():
+        y = ops.embedding_lookup(fwd.make_dual(w, tw), ids, 0.5)
+        assert y.requires_grad == requires_grad
+        primal, tangent = fwd.unpack_dual(y)
+        assert torch.equal(primal, ops.embedding_lookup(w, ids, 0.5))
+        assert torch.equal(tangent, want[0])
+        tangent = fwd.unpack_dual(ops.embedding_lookup_grad(fwd.make_dual(dy, tdy), ids, V, 0.5,
+                                                            3)).tangent
+        assert torch.equal(tangent, want[1])
+        if requires_grad:  # forward over reverse
+            g, = torch.autograd.grad(y, w, fwd.make_dual(dy, tdy))
+            assert torch.equal(fwd.unpack_dual(g).tangent,
+                               ops.embedding_lookup_grad(tdy, ids, V, 0.5))
+
+
+def test_forward_mode_is_refused_where_there_is_no_derivative():
+    import torch.autograd.forward_ad as fwd
+    w, _, dy = inputs(9)
+    kept = w.clone()
+    with fwd.dual_level():
+        dual = fwd.make_dual(w, torch.ones_like(w))
+        for call in (lambda: ops.global_norm([dy, dual]),
+                     lambda: ops.clip_by_global_norm([dual], 1.0),
+                     lambda: ops.clip_by_global_norm([w], 1.0, out=[dual]),
+                     lambda: ops.clip_by_global_norm_([dual], 1.0)):
+            for guard in (torch.enable_grad, torch.no_grad):
+                with guard(), pytest.raises(ValueError, match="tangent"):
+                    call()
+    assert torch.equal(w, kept)
+    assert float(ops.global_norm([w])) > 0
+
+
+def test_functional_transforms():
+    w, ids, c = inputs(10)
+    t = torch.randn_like(w)
+
+    def f(w):
+        return (ops.embedding_lookup(w, ids, 0.5, 3) * c).sum()
+
+    want = ops.embedding_lookup_grad(c, ids, V, 0.5, 3)
+    assert torch.equal(torch.func.grad(f)(w), want)
+    y, dy = torch.func.jvp(lambda w: ops.embedding_lookup(w, ids, 2.0), (w,), (t,))
+    assert torch.equal(y, ops.embedding_lookup(w, ids, 2.0))
+    assert torch.equal(dy, ops.embedding_lookup(t, ids, 2.0))
+    _, back = torch.func.vjp(lambda w: ops.embedding_lookup(w, ids, 2.0), w)
+    assert torch.equal(back(c)[0], ops.embedding_lookup_grad(c, ids, V, 2.0))
+    for a, b in zip(torch.func.vmap(lambda i: ops.embedding_lookup(w, i))(ids.view(5, 10)),
+                    ids.view(5, 10)):
+        assert torch.equal(a, ops.embedding_lookup(w, b))
+    many = torch.stack([w, t])
+    for a, b in zip(torch.func.vmap(lambda w: ops.embedding_lookup(w, ids))(many), many):
+        assert torch.equal(a, ops.embedding_lookup(b, ids))
+    per = torch.func.vmap(torch.func.grad(lambda w, i: (ops.embedding_lookup(w, i) * c[:10]).sum()),
+                          (None, 0))(w, ids.view(5, 10))
+    for a, b in zip(per, ids.view(5, 10)):
+        assert torch.equal(a, ops.embedding_lookup_grad(c[:10], b, V))
+
+
+def test_double_backward_is_refused():
+    w, ids, c = inputs(11)
+    w.requires_grad_(True)
+    y = ops.embedding_lookup(w, ids)
+    g, = torch.autograd.grad(y.square().sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError, match="once, not twice"):
+        g.sum().backward()
+    # a gradient that nothing differentiable went into is a constant, as torch's own
+    y = ops.embedding_lookup(w, ids)
+    g, = torch.autograd.grad(y, w, c, create_graph=True)
+    assert not g.requires_grad and torch.equal(g, ops.embedding_lookup_grad(c, ids, V))
+    with pytest.raises(RuntimeError, match="once, not twice"):
+        torch.func.grad(lambda a: torch.func.grad(
+            lambda b: ops.embedding_lookup(b, ids).square().sum())(a).sum())(w.detach())
+
+
+def test_an_undefined_gradient_is_zero():
+    class Stop(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, y):
+            return y.clone()
+
+        @staticmethod
+        def backward(ctx, dy):
+            return None
+
+    w, ids, _ = inputs(12)
+    w = w.bfloat16().requires_grad_(True)
+    g, = torch.autograd.grad(Stop.apply(ops.embedding_lookup(w, ids)).sum(), w)
+    assert g.dtype == w.dtype and g.shape == w.shape and not g.any()
