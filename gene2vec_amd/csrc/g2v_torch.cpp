@@ -342,6 +342,9 @@ at::Tensor embedding_lookup_grad(py::handle dy_, py::handle ids_, py::handle voc
                                  double scale, py::handle padding_idx, py::handle dtype) {
   const at::Tensor& dy = tensor(dy_, "dy");
   on_gpu(dy, "dy");
+  if (ag::compute_requires_grad(dy))
+    refuse("embedding_lookup_grad is not differentiable: pass a dy that requires no gradient, or "
+           "call it under no_grad()");
   const at::Tensor& ids = tensor(ids_, "ids");
   on_gpu(ids, "ids");
   const at::ScalarType type = result_type(dtype, dy.scalar_type());

@@ -63,6 +63,8 @@ def embedding_lookup_grad(dy, ids, vocab_size, scale=1.0, padding_idx=None, dtyp
     dy  ids.shape + (D,), float32, float16 or bfloat16, any strides (rows that
         are not contiguous are copied); dtype of the result: None = dy's.
     The sums are fp32 in a fixed order, without atomics, and rounded once.
+    Not differentiable, but for forward mode in dy: a dy that requires a gradient
+    is refused in grad mode.
     """
     return _x.embedding_lookup_grad(dy, ids, vocab_size, scale, padding_idx, dtype)
 

@@ -215,3 +215,16 @@ def test_an_undefined_gradient_is_zero():
     w = w.bfloat16().requires_grad_(True)
     g, = torch.autograd.grad(Stop.apply(ops.embedding_lookup(w, ids)).sum(), w)
     assert g.dtype == w.dtype and g.shape == w.shape and not g.any()
+
+
+def test_the_gradient_refuses_a_dy_that_requires_one():
+    _, ids, dy = inputs(13)
+    want = ops.embedding_lookup_grad(dy, ids, V)
+    dy.requires_grad_(True)
+    with pytest.raises(ValueError, match="not differentiable"):
+        ops.embedding_lookup_grad(dy, ids, V)
+    with torch.no_grad():
+        assert torch.equal(ops.embedding_lookup_grad(dy, ids, V), want)
+    assert torch.equal(ops.embedding_lookup_grad(dy.detach(), ids, V), want)
+    with pytest.raises(RuntimeError, match="once, not twice"):  # past the Python entry
+        torch.ops.g2v.embedding_lookup_grad(dy, ids, V, 1.0, -1, torch.float32).sum().backward()
