@@ -15,10 +15,12 @@
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -31,6 +33,7 @@
 #include <stdexcept>
 #include <string>
 #include <tuple>
+#include <unordered_set>
 #include <vector>
 
 #include "g2v.h"
@@ -243,15 +246,30 @@ namespace ag = torch::autograd;
 // A leaf's gradient is accumulated on the stream that its live graph was built
 // on.  Where that is the default stream, which no capture can take in, a captured
 // backward pass would end the capture, or the process: refused here, before
-// anything is recorded.
+// anything is recorded.  The leaves are params itself or what it was computed from.
 void check_capture(const at::Tensor& params) {
+  const c10::DeviceGuard guard(params.device());  // the capture of its stream is asked for
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-  const std::shared_ptr<ag::Node> node = ag::impl::try_get_grad_accumulator(params);
-  if (!node) return;
-  const auto stream = node->stream();
-  if (stream && stream->id() == c10::hip::getDefaultHIPStream(params.device().index()).id())
-    refuse("params: a graph of this leaf from the default stream is still alive (its loss, "
-           "say); drop it before capturing");
+  const auto check = [](ag::Node& leaf) {
+    const auto stream = leaf.stream();
+    if (stream &&
+        stream->id() == c10::hip::getDefaultHIPStream(stream->device_index()).id())
+      refuse("params: a graph of this leaf, or of one that it was computed from, is still alive "
+             "from the default stream (a loss, say); drop it before capturing");
+  };
+  if (!params.grad_fn()) {
+    if (const auto leaf = ag::impl::try_get_grad_accumulator(params)) check(*leaf);
+    return;
+  }
+  std::vector<ag::Node*> todo{params.grad_fn().get()};
+  std::unordered_set<ag::Node*> seen(todo.begin(), todo.end());
+  while (!todo.empty()) {
+    ag::Node* node = todo.back();
+    todo.pop_back();
+    if (dynamic_cast<ag::AccumulateGrad*>(node)) check(*node);
+    for (const ag::Edge& e : node->next_edges())
+      if (e.function && seen.insert(e.function.get()).second) todo.push_back(e.function.get());
+  }
 }
 
 struct EmbeddingLookupBackward : public ag::Node {

@@ -16,9 +16,10 @@ the same bits.  Tensors and values that do not fit raise ``ValueError``
 before anything runs, the library's own errors ``_native.G2VError``.
 
 A lookup in a table that requires its gradient is captured only while no graph
-of that leaf from the default stream lives (``del`` the loss of earlier steps):
-torch accumulates on the stream that graph was built on, and the default stream
-ends a capture, so the call raises ``ValueError`` then.
+of that leaf, or of a leaf that the table was computed from, lives from the
+default stream (``del`` the loss of earlier steps): torch accumulates on the
+stream that graph was built on, and the default stream ends a capture, so the
+call raises ``ValueError`` then.
 """
 from __future__ import annotations
 
