@@ -10,8 +10,9 @@ pipeline, architecture, initialisers and optimiser:
          myFit (lines without 2 genes stay [1, 1]), one-hot labels
   embed  GGIPNN_util.load_embedding_vectors: U(-0.25, 0.25) then rows found in
          the .txt (line.split()); frozen unless train_embedding=True
-         (GGIPNN.py:19-21).  On the GPU the lookup and the gradient of its
-         table are ``ops.embedding_lookup``, on the CPU torch indexing
+         (GGIPNN.py:19-21).  A frozen table is read by torch indexing; on the
+         GPU the lookup of a trained one, and its gradient, are
+         ``ops.embedding_lookup``
   model  GGIPNN.py:25-69 -- concat(2 x D) -> 100 -> 100 -> 10 -> 2, ReLU,
          dropout keep 0.5 after each hidden layer, biases 0.1, weights
          variance_scaling (factor 2, fan_in, truncated normal)
@@ -140,7 +141,7 @@ def build_model(vocab_size, emb, embedding_size, device, gen, train_embedding=Fa
                 self.bs.append(nn.Parameter(torch.full((b,), 0.1, device=device)))
 
         def forward(self, x, keep_prob):
-            if self.W.is_cuda:
+            if train_embedding and self.W.is_cuda:
                 from . import ops
                 h = ops.embedding_lookup(self.W, x)
             else:
