@@ -12,7 +12,7 @@ pipeline, architecture, initialisers and optimiser:
          the .txt (line.split()); frozen unless train_embedding=True
          (GGIPNN.py:19-21).  A frozen table is read by torch indexing; on the
          GPU the lookup of a trained one, and its gradient, are
-         ``ops.embedding_lookup``
+         ``ops.embedding_lookup`` (float64: torch indexing)
   model  GGIPNN.py:25-69 -- concat(2 x D) -> 100 -> 100 -> 10 -> 2, ReLU,
          dropout keep 0.5 after each hidden layer, biases 0.1, weights
          variance_scaling (factor 2, fan_in, truncated normal)
@@ -122,7 +122,24 @@ def clip_gradients_(params, clip_norm):
     return norm.float()
 
 
+def _trained_rows(W, x):
+    """W's rows by token; a token outside the table has none, on either device:
+    zeros, and no gradient.  The operators take float32, float16 and bfloat16
+    with tokens beside the table, torch indexing the rest"""
+    import torch
+    if (W.is_cuda and x.device == W.device and x.dtype in (torch.int32, torch.int64)
+            and W.dtype in (torch.float32, torch.float16, torch.bfloat16)):
+        from . import ops
+        return ops.embedding_lookup(W, x)
+    x = x.to(W.device, torch.int64)
+    there = (x >= 0) & (x < W.shape[0])
+    return torch.where(there[..., None], W[torch.where(there, x, 0)], 0.0)
+
+
 def build_model(vocab_size, emb, embedding_size, device, gen, train_embedding=False):
+    """the classifier; forward(tokens, keep_prob) takes tokens [batch, 2].  A
+    frozen table is indexed as torch indexes (-1 is the last row, a token outside
+    is an error); a trained one has zero rows for tokens outside [0, vocab_size)"""
     import torch
     import torch.nn as nn
 
@@ -141,12 +158,7 @@ def build_model(vocab_size, emb, embedding_size, device, gen, train_embedding=Fa
                 self.bs.append(nn.Parameter(torch.full((b,), 0.1, device=device)))
 
         def forward(self, x, keep_prob):
-            if train_embedding and self.W.is_cuda:
-                from . import ops
-                h = ops.embedding_lookup(self.W, x)
-            else:
-                h = self.W[x]
-            h = h.reshape(x.shape[0], -1)
+            h = (_trained_rows(self.W, x) if train_embedding else self.W[x]).reshape(x.shape[0], -1)
             for i in range(3):
                 h = torch.relu(h @ self.ws[i] + self.bs[i])
                 if keep_prob < 1.0:

@@ -77,3 +77,35 @@ def test_frozen_classifier_keeps_torch_indexing():
     g, = torch.autograd.grad(m(x.cuda(), 1.0).square().sum(), m.W, create_graph=True)
     g.square().sum().backward()
     assert math.isfinite(float(m.W.grad.sum()))
+
+
+def loss_and_grads(m, x):
+    t = torch.arange(len(x), device=m.W.device) % 2
+    loss = torch.nn.functional.cross_entropy(m(x, 1.0), t)
+    return [loss.detach()] + list(torch.autograd.grad(loss, list(m.parameters())))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("place", ["beside", "int32", "host"])
+def test_trained_classifier_is_the_same_on_both_devices(dtype, place):
+    """tokens outside the table among them"""
+    x = tokens(5)
+    x[0], x[1, 0], x[2, 1] = -1, V, 2**31 - 1
+    given = {"beside": x.cuda(), "int32": x.cuda().int(), "host": x}[place]
+    got = loss_and_grads(model("cuda", True, dtype), given)
+    want = loss_and_grads(model("cpu", True, dtype), x)
+    for a, b in zip(got, want):
+        assert a.dtype == b.dtype
+        close(a, b, dtype)
+
+
+def test_trained_classifier_is_traced():
+    m, x = model("cuda", True), tokens().cuda()
+    traced = torch.jit.trace(Keep1(m), (x,))
+    for seed in (0, 1, 2):
+        x = tokens(seed).cuda()
+        x[seed] = V
+        assert torch.equal(traced(x), m(x, 1.0))
+    g, = torch.autograd.grad(traced(x).square().sum(), m.W)
+    w, = torch.autograd.grad(m(x, 1.0).square().sum(), m.W)
+    assert torch.equal(g, w)
