@@ -112,13 +112,15 @@ def clip_gradients_(params, clip_norm):
     grads = [p.grad for p in params if p.grad is not None]
     if not grads:
         raise ValueError("no parameter has a gradient")
-    if all(g.is_cuda for g in grads):
+    if all(g.is_cuda and g.dtype in (torch.float32, torch.float16, torch.bfloat16)
+           for g in grads):
         from . import ops
         return ops.clip_by_global_norm_(grads, clip_norm)
     norm = torch.sqrt(sum(g.double().square().sum() for g in grads))
     factor = torch.where(norm.isfinite(), clip_norm / norm.clamp(min=clip_norm), math.nan)
-    for g in grads:
-        g.mul_(factor.to(g.dtype))
+    f32 = factor.float().double()
+    for g in grads:  # fp64: the gradients' own type; else fp32, whatever theirs
+        g.copy_(g.double() * (factor if g.dtype == torch.float64 else f32))
     return norm.float()
 
 
