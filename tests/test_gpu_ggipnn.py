@@ -109,3 +109,85 @@ def test_trained_classifier_is_traced():
     g, = torch.autograd.grad(traced(x).square().sum(), m.W)
     w, = torch.autograd.grad(m(x, 1.0).square().sum(), m.W)
     assert torch.equal(g, w)
+
+
+# ---- train_and_auc: what its arguments change ---------------------------------------------
+def train(tmp_path, monkeypatch, device, **kw):
+    """train_and_auc on small random splits from the same weights on every device,
+    without dropout: (table before, model after, gradients at every step, AUC)"""
+    rng = np.random.RandomState(1)
+    genes = [f"G{i}" for i in range(V)]
+    for name, n in (("train", 600), ("valid", 10), ("test", 80)):
+        a, b = rng.randint(0, V - 5, n), rng.randint(0, V, n)  # the last genes are rare
+        (tmp_path / f"{name}_text.txt").write_text(
+            "\n".join(f"{genes[i]} {genes[j]}" for i, j in zip(a, b)))
+        (tmp_path / f"{name}_label.txt").write_text("\n".join(map(str, (a + b) % 2)))
+    emb = tmp_path / "emb.txt"
+    emb.write_text("".join(g + "\t" + "".join(f"{v} " for v in rng.randn(D)) + "\n" for g in genes))
+    seen = {"steps": []}
+    build = G.build_model
+
+    def spy_build(vocab, e, size, dev, gen, trained=False):
+        m = build(vocab, e, size, "cpu", torch.Generator().manual_seed(9), trained).to(dev)
+        seen["model"], seen["before"] = m, m.W.detach().clone()
+        return m
+
+    step = torch.optim.Adam.step
+
+    def spy_step(self, *a, **k):
+        seen["params"] = [p for group in self.param_groups for p in group["params"]]
+        seen["steps"].append([p.grad.detach().cpu().double().clone() for p in seen["params"]])
+        return step(self, *a, **k)
+
+    with monkeypatch.context() as mp:
+        mp.setattr(G, "build_model", spy_build)
+        mp.setattr(torch.optim.Adam, "step", spy_step)
+        seen["auc"] = G.train_and_auc(str(emb), str(tmp_path), seed=0, embedding_size=D,
+                                      device=device, keep_prob=1.0, **kw)
+    return seen
+
+
+def norms(seen):
+    return [math.sqrt(sum(float(g.square().sum()) for g in grads)) for grads in seen["steps"]]
+
+
+def test_training_leaves_a_frozen_table_alone(tmp_path, monkeypatch):
+    seen = train(tmp_path, monkeypatch, "cuda")
+    assert torch.equal(seen["model"].W, seen["before"]) and seen["model"].W.grad is None
+    assert not any(p is seen["model"].W for p in seen["params"]) and len(seen["steps"]) == 5
+
+
+@pytest.mark.parametrize("clip", [None, 0.05])
+def test_training_moves_its_table_as_on_the_cpu(tmp_path, monkeypatch, clip):
+    got = train(tmp_path, monkeypatch, "cuda", train_embedding=True, clip_norm=clip)
+    want = train(tmp_path, monkeypatch, "cpu", train_embedding=True, clip_norm=clip)
+    assert any(p is got["model"].W for p in got["params"]) and len(got["steps"]) == 5
+    assert torch.equal(got["before"].cpu(), want["before"])
+    # the first step's gradients; later ones follow Adam's division by their own
+    # size, which makes the smallest differences whole steps
+    for a, b in zip(got["steps"][0], want["steps"][0]):
+        close(a, b)
+    # Adam's first step is lr * g / (|g| + eps): rows with a gradient move
+    moved = (got["model"].W.detach() != got["before"]).any(1).cpu()
+    assert bool(moved[got["steps"][0][0].abs().amax(1) > 1e-6].all())
+    assert int(moved.sum()) > V // 2
+    # the table's gradient at the first step is dense where tokens are, zero elsewhere
+    assert torch.equal(got["steps"][0][0].abs().sum(1) > 0, want["steps"][0][0].abs().sum(1) > 0)
+    free = norms(got if clip is None else train(tmp_path, monkeypatch, "cuda",
+                                                train_embedding=True))
+    assert max(free) > 0.05  # the bound below acts
+    if clip is not None:
+        # the norm rounds once, factor and product once each: 3 u over the bound
+        assert max(norms(got)) <= clip * (1 + 4 * 2**-24)
+        assert norms(got)[0] == pytest.approx(clip, rel=4 * 2**-24)
+    from sklearn import metrics
+    m = got["model"]
+    with torch.no_grad():
+        rows = [ln.split(" ") for ln in (tmp_path / "test_text.txt").read_text().splitlines()]
+        lines = [ln for n in ("train", "valid", "test")
+                 for ln in (tmp_path / f"{n}_text.txt").read_text().splitlines()]
+        d = G.my_fit_dict(lines)
+        x = torch.tensor([[d[a], d[b]] for a, b in rows], device="cuda")
+        s = torch.softmax(m(x, 1.0), 1)[:, 1].cpu().numpy()
+    y = [int(v) for v in (tmp_path / "test_label.txt").read_text().split()]
+    assert got["auc"] == float(metrics.roc_auc_score(y, s))
