@@ -1,8 +1,9 @@
 // g2v_gradnorm.hip -- the global norm of a list of gradients, and clipping.
 //
 //   norm = sqrt(sum over tensors and elements of g^2)
-//   clip: dst = g * (clip / max(norm, clip)); NaN everywhere when the norm is
-//         not finite (an overflow is not hidden)
+//   clip: dst = g * (clip / max(norm, clip)); NaN everywhere when an element is
+//         not finite (an overflow is not hidden).  A finite norm beyond fp32 is
+//         returned as infinity, and its elements are clipped.
 //
 // The squares are formed and added in fp64: an fp32 sum would overflow from
 // elements of 1.8e19 on and lose the small tensors beside the large ones, and
@@ -196,13 +197,17 @@ __global__ __launch_bounds__(kThreads) void k_clip(A a, const double* __restrict
                                                    float* __restrict__ norm) {
   const double nrm = sqrt(sum_partials(partial, np));
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)nrm;
-  const float f = (float)(nrm < INFINITY ? clip / (nrm > clip ? nrm : clip) : NAN);
-  if (in_place && f == 1.f) return;  // within the bound
+  const double factor = nrm < INFINITY ? clip / (nrm > clip ? nrm : clip) : NAN;
+  // a factor below fp32's normal numbers (a norm 10^38 times the bound) would keep
+  // few of its bits there: its exponent is applied apart, after the product
+  int e = 0;
+  const float f = (float)(factor < 0x1p-126 ? frexp(factor, &e) : factor);
+  if (in_place && f == 1.f && e == 0) return;  // within the bound
   for_elements<true>(a, [&](int t, auto z, int64_t at, auto& x) {
     using T = decltype(z);
     constexpr int N = sizeof x / sizeof x[0];
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] *= f;
+    for (int i = 0; i < N; ++i) x[i] = ldexpf(x[i] * f, e);
     g2v::store_vec_nt<T, N>(static_cast<T*>(a.dst[t]) + at, x);
   });
 }

@@ -105,7 +105,8 @@ def _variance_scaling_(w, gen):
 
 def clip_gradients_(params, clip_norm):
     """scale the gradients in place by clip_norm / max(norm, clip_norm), norm
-    over all of them (NaN everywhere if it is not finite); returns the norm"""
+    over all of them (NaN everywhere if an element is not finite); returns the
+    norm in fp32, infinite where it is beyond that"""
     import torch
     if not 0.0 < clip_norm < math.inf:
         raise ValueError(f"clip_norm must be positive and finite, not {clip_norm}")
@@ -118,7 +119,8 @@ def clip_gradients_(params, clip_norm):
         return ops.clip_by_global_norm_(grads, clip_norm)
     norm = torch.sqrt(sum(g.double().square().sum() for g in grads))
     factor = torch.where(norm.isfinite(), clip_norm / norm.clamp(min=clip_norm), math.nan)
-    f32 = factor.float().double()
+    # 24 bits of the factor, also where it is below fp32's normal numbers
+    f32 = torch.where(factor < 2.0**-126, factor, factor.float().double())
     for g in grads:  # fp64: the gradients' own type; else fp32, whatever theirs
         g.copy_(g.double() * (factor if g.dtype == torch.float64 else f32))
     return norm.float()

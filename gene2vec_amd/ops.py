@@ -89,8 +89,10 @@ def clip_by_global_norm(t_list, clip_norm, out=None):
     out  None: new tensors; else a list of tensors of the same shapes, types
          and strides to write, apart from each other and from the inputs, or
          the input itself in its own place.  ``None`` entries stay ``None``.
-    A norm that is not finite makes every element NaN, so that an overflow is
-    not taken for a step of length zero.
+    An element that is infinite or NaN makes every element NaN, so that an
+    overflow is not taken for a step of length zero.  The factor is of the fp64
+    norm: one that is finite but beyond fp32 is returned as infinity, and the
+    tensors are clipped all the same.
     """
     return _x.clip_by_global_norm(t_list, clip_norm, out)
 

@@ -504,9 +504,11 @@ int g2v_global_norm(int device, const void *const *tensors, const int64_t *numel
                     int64_t workspace_bytes, void *stream);
 
 /* dst[t] = src[t] * (clip_norm / max(norm, clip_norm)), the factor rounded to
- * fp32 and the product once to the type; *norm as above, before the
- * clipping.  A norm that is not finite makes every element NaN.  dst[t] ==
- * src[t] clips in place; any other overlap is refused. */
+ * 24 bits whatever its size, the product formed in fp32 and rounded to the type;
+ * *norm as above, before the clipping.  An element that is infinite or NaN makes
+ * every element NaN.  The factor is of the fp64 norm: where that is finite but
+ * beyond fp32, *norm is infinite and the elements are clipped all the same.
+ * dst[t] == src[t] clips in place; any other overlap is refused. */
 int g2v_clip_global_norm(int device, const void *const *src, void *const *dst,
                          const int64_t *numel, const int32_t *types, int64_t n, double clip_norm,
                          float *norm, void *workspace, int64_t workspace_bytes, void *stream);
