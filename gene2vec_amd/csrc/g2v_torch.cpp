@@ -389,11 +389,11 @@ struct List {
     src.reserve(n);
     numel.reserve(n);
     types.reserve(n);
-    for (const at::Tensor& t : tensors) {
-      on_gpu(t, what);
-      if (t.device() != tensors[0].device())
-        refuse(std::string(what) + ": tensors on " + tensors[0].device().str() + " and " +
-               t.device().str());
+    on_gpu(tensors[0], what);
+    const c10::Device where = tensors[0].device();
+    for (const at::Tensor& t : tensors) {  // other layouts have no kernel to come here by
+      if (t.device() != where)
+        refuse(std::string(what) + ": tensors on " + where.str() + " and " + t.device().str());
       const int type = type_code(t.scalar_type());
       if (type < 0)
         refuse(std::string(what) + ": tensors must be float32, float16 or bfloat16, not " +
@@ -461,7 +461,6 @@ at::Tensor clip_out_cuda(at::TensorList t_list, double clip_norm, at::TensorList
            std::to_string(t_list.size()) + " tensors");
   for (size_t i = 0; i < out.size(); ++i) {
     const at::Tensor &o = out[i], &t = t_list[i];
-    on_gpu(o, "clip_by_global_norm: out");
     if (o.sizes() != t.sizes() || o.scalar_type() != t.scalar_type() ||
         o.device() != t.device() ||
         !((o.is_contiguous() && t.is_contiguous()) || o.strides() == t.strides()))
@@ -479,6 +478,7 @@ at::Tensor clip_inplace_cuda(at::TensorList t_list, double clip_norm) {
 void no_derivative(at::TensorList tensors, const char* what) {
   const bool grad = at::GradMode::is_enabled();
   for (const at::Tensor& t : tensors) {
+    if (!t.unsafeGetTensorImpl()->autograd_meta()) continue;  // plain data, as most are
     if (grad && t.requires_grad())
       refuse(std::string(what) +
              " is not differentiable: pass gradients, or call it under no_grad()");
