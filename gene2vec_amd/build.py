@@ -27,15 +27,18 @@ HEADERS = [os.path.join(CSRC, "g2v_internal.h"), os.path.join(CSRC, "g2v_device.
            os.path.join(CSRC, "g2v_ops.h"), os.path.join(CSRC, "g2v_counts.h"),
            os.path.join(ROOT, "include", "g2v.h")]
 ARCH = "gfx950"
+# what every unit is compiled with, but for include paths and -D
+COMPILE_FLAGS = (f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
+                 # IEEE semantics: every fused multiply-add in the kernels is explicit
+                 "-ffp-contract=off", "-munsafe-fp-atomics", "-pthread")
+# no packed fp32 arithmetic (v_pk_add / mul / fma_f32), which the compiler forms
+# from ordinary float code and which is not relied on here.  Every device unit;
+# the host pass warns that it does not know the feature, which is harmless
+DEVICE_FLAGS = ("-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops")
 # k_sgns_atomic's store-or-atomics choice per row is a uniform if / else that
 # must stay a diamond for the loop head to wait with vmcnt(#row instructions)
 # instead of vmcnt(0) (g2v_sgns_atomic.hip; tests/test_kernel_isa.py)
-SGNS_KERNEL_FLAGS = ("-mllvm", "-structurizecfg-skip-uniform-regions=true")
-# no packed fp32 arithmetic (v_pk_add / mul / fma_f32): the compiler forms it
-# from ordinary float code, and some of its forms have given wrong results on
-# MI355X.  Every device unit; the host pass warns that it does not know the
-# feature, which is harmless
-DEVICE_FLAGS = ("-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops")
+SGNS_KERNEL_FLAGS = (*DEVICE_FLAGS, "-mllvm", "-structurizecfg-skip-uniform-regions=true")
 # the sources that determine k_sgns_atomic's code (bench.py accepts a PMC
 # traffic profile only when it was measured on this exact kernel code AND the
 # same launch layout: grid and stripe tiers, recorded beside the hash)
@@ -43,14 +46,23 @@ KERNEL_SOURCES = [os.path.join(CSRC, s) for s in
                   ("g2v_sgns_atomic.hip", "g2v_device.h", "g2v_internal.h")]
 
 
+def unit_flags(src: str) -> tuple:
+    """the code generation flags of one unit beyond COMPILE_FLAGS"""
+    if src == "g2v_sgns_atomic.hip":
+        return SGNS_KERNEL_FLAGS
+    return DEVICE_FLAGS if src.endswith(".hip") else ()
+
+
 def kernel_source_hash() -> str:
-    """sha256 (first 16 hex digits) of KERNEL_SOURCES, in that order"""
+    """sha256 (first 16 hex digits) of KERNEL_SOURCES, in that order, and of the
+    flags they are compiled with"""
     import hashlib
     h = hashlib.sha256()
     for p in KERNEL_SOURCES:
         h.update(os.path.basename(p).encode() + b"\0")
         with open(p, "rb") as f:
             h.update(f.read())
+    h.update("\0".join((*COMPILE_FLAGS, *unit_flags("g2v_sgns_atomic.hip"))).encode())
     return h.hexdigest()[:16]
 
 
@@ -90,18 +102,14 @@ def build(force: bool = False, verbose: bool = False, ablations: bool = False,
         out, objdir = ABLATIONS_LIB, os.path.join(HERE, "build", "ablations")
     else:
         out, objdir = LIB, os.path.join(HERE, "build")
-    flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
-             # IEEE semantics: every fused multiply-add in the kernels is explicit
-             "-ffp-contract=off", "-munsafe-fp-atomics", "-pthread",
-             "-I", os.path.join(ROOT, "include"), "-I", CSRC]
+    flags = [*COMPILE_FLAGS, "-I", os.path.join(ROOT, "include"), "-I", CSRC]
     if ablations:
         flags.append("-DG2V_ABLATIONS")
     flags += [f"-D{d}" for d in defines]
     # the objects' compile flags are part of their key: a stamp in
     # the object directory; another flag set rebuilds every object there
     stamp = os.path.join(objdir, "flags.stamp")
-    key = " ".join(flags + ["|"] + list(DEVICE_FLAGS) + list(SGNS_KERNEL_FLAGS)
-                   + list(kernel_flags))
+    key = " ".join([*flags, "|", *DEVICE_FLAGS, "|", *SGNS_KERNEL_FLAGS, *kernel_flags])
     old_key = open(stamp).read() if os.path.exists(stamp) else None
     if old_key is not None and old_key != key:
         force = True
@@ -117,9 +125,9 @@ def build(force: bool = False, verbose: bool = False, ablations: bool = False,
         if (not force and os.path.exists(objs[i])
                 and all(os.path.getmtime(d) <= os.path.getmtime(objs[i]) for d in deps)):
             return ""
-        kf = (list(SGNS_KERNEL_FLAGS) + list(kernel_flags)) if src == "g2v_sgns_atomic.hip" else []
-        df = DEVICE_FLAGS if src.endswith(".hip") else ()
-        cmd = [hipcc(), *flags, *df, *kf, *defs, "-c", os.path.join(CSRC, src), "-o", objs[i]]
+        kf = kernel_flags if src == "g2v_sgns_atomic.hip" else ()
+        cmd = [hipcc(), *flags, *unit_flags(src), *kf, *defs, "-c", os.path.join(CSRC, src),
+               "-o", objs[i]]
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
         r = subprocess.run(cmd, capture_output=True, text=True)
