@@ -155,32 +155,53 @@ TORCH_LIB = os.path.join(HERE, "_g2v_torch.so")
 TORCH_SOURCE = os.path.join(CSRC, "g2v_torch.cpp")
 
 
-def build_torch(force: bool = False, verbose: bool = False) -> str:
-    """the operators' Python module (_g2v_torch.so): host code against the
-    installed torch and libg2v.so, which is built before"""
-    deps = (TORCH_SOURCE, os.path.join(ROOT, "include", "g2v.h"), __file__)
-    if (not force and os.path.exists(TORCH_LIB)
-            and all(os.path.getmtime(d) <= os.path.getmtime(TORCH_LIB) for d in deps)):
-        return TORCH_LIB
+TORCH_STAMP = os.path.join(HERE, "build", "torch.stamp")
+
+
+def torch_command() -> list:
     import sysconfig
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
     rocm = os.path.dirname(os.path.dirname(hipcc()))
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-pthread", "-fvisibility=hidden",
-           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-I", os.path.join(ROOT, "include"),
-           *(f"-isystem{d}" for d in (*include_paths(), sysconfig.get_paths()["include"],
-                                      os.path.join(rocm, "include"))),
-           TORCH_SOURCE, "-L", HERE, "-lg2v", *(f"-L{d}" for d in library_paths()),
-           "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_hip", "-lc10",
-           "-Wl,-rpath,$ORIGIN", "-o", TORCH_LIB + ".tmp"]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-pthread", "-fvisibility=hidden",
+            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            "-I", os.path.join(ROOT, "include"),
+            *(f"-isystem{d}" for d in (*include_paths(), sysconfig.get_paths()["include"],
+                                       os.path.join(rocm, "include"))),
+            TORCH_SOURCE, "-L", HERE, "-lg2v", *(f"-L{d}" for d in library_paths()),
+            "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_hip", "-lc10",
+            "-Wl,-rpath,$ORIGIN", "-o", TORCH_LIB + ".tmp"]
+
+
+def torch_key() -> str:
+    """what _g2v_torch.so is made from: the sources, torch, the command"""
+    import hashlib
+    import torch
+    h = hashlib.sha256()
+    for p in (TORCH_SOURCE, os.path.join(ROOT, "include", "g2v.h")):
+        with open(p, "rb") as f:
+            h.update(f.read() + b"\0")
+    return "\n".join([h.hexdigest(), torch.__version__, *torch_command()])
+
+
+def build_torch(force: bool = False, verbose: bool = False) -> str:
+    """the operators' Python module (_g2v_torch.so): host code against the
+    installed torch and libg2v.so, which is built before"""
+    key = torch_key()
+    if (not force and os.path.exists(TORCH_LIB) and os.path.exists(TORCH_STAMP)
+            and open(TORCH_STAMP).read() == key):
+        return TORCH_LIB
+    cmd = torch_command()
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode:
         raise RuntimeError(f"g++ failed on {TORCH_SOURCE}:\n{r.stderr}")
     os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+    os.makedirs(os.path.dirname(TORCH_STAMP), exist_ok=True)
+    with open(TORCH_STAMP, "w") as f:
+        f.write(key)
     return TORCH_LIB
 
 

@@ -26,6 +26,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
+#include <torch/version.h>
 
 #include <cmath>
 #include <cstdint>
@@ -632,7 +633,9 @@ PYBIND11_MODULE(_g2v_torch, m) {
       PyErr_SetString(PyExc_ValueError, e.what_without_backtrace());
     }
   });
-  m.def("abi_version", &g2v_abi_version);
+  // what this file was compiled against, not what libg2v answers at run time
+  m.def("abi_version", [] { return G2V_ABI_VERSION; });
+  m.def("torch_version", [] { return TORCH_VERSION; });
   m.def("embedding_lookup", [](py::handle p, py::handle i, double s, py::handle pad,
                                py::handle d) { return wrap(embedding_lookup(p, i, s, pad, d)); });
   m.def("embedding_lookup_grad",

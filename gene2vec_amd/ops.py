@@ -23,7 +23,7 @@ call raises ``ValueError`` then.
 """
 from __future__ import annotations
 
-import torch  # noqa: F401  (its libraries, and its HIP runtime, come first)
+import torch  # (its libraries, and its HIP runtime, come first)
 
 from . import _native as N
 
@@ -34,9 +34,12 @@ except ImportError as e:
     raise N.NativeLibraryError(
         f"gene2vec_amd/_g2v_torch.so is missing or does not load ({e}): build it with "
         "`python -m gene2vec_amd.build`") from e
-if _x.abi_version() != N.ABI_VERSION:
-    raise N.NativeLibraryError("_g2v_torch.so was built for another libg2v: "
-                               "`python -m gene2vec_amd.build --force`")
+if (_x.abi_version() != N.ABI_VERSION
+        or _x.torch_version() != torch.__version__.split("+")[0]):
+    raise N.NativeLibraryError(
+        f"_g2v_torch.so was built for libg2v's ABI {_x.abi_version()} and torch "
+        f"{_x.torch_version()}, not {N.ABI_VERSION} and {torch.__version__}: "
+        "`python -m gene2vec_amd.build --force`")
 
 
 def embedding_lookup(params, ids, scale=1.0, padding_idx=None, dtype=None):
