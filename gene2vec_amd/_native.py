@@ -198,12 +198,18 @@ def lib():
         L = C.CDLL(LIB_PATH)
     except OSError as e:  # pragma: no cover - depends on the ROCm runtime
         raise NativeLibraryError(f"failed to load {LIB_PATH}: {e}") from e
+    rebuild = "rebuild it with `python -m gene2vec_amd.build --force`"
+    missing = [name for name in SIGNATURES if not hasattr(L, name)]
+    if "g2v_abi_version" in missing or L.g2v_abi_version() != ABI_VERSION:
+        raise NativeLibraryError(f"libg2v ABI version mismatch: {LIB_PATH} is not of version "
+                                 f"{ABI_VERSION}; {rebuild}")
+    if missing:
+        raise NativeLibraryError(f"{LIB_PATH} is of an older tree, without {', '.join(missing)}; "
+                                 f"{rebuild}")
     for name, (res, args) in SIGNATURES.items():
         f = getattr(L, name)
         f.restype = res
         f.argtypes = args
-    if L.g2v_abi_version() != ABI_VERSION:
-        raise NativeLibraryError("libg2v ABI version mismatch")
     _lib = L
     return L
 
