@@ -137,9 +137,12 @@ class DeviceScope {
     if (!(cond)) return g2v::op_fail((code), __VA_ARGS__); \
   } while (0)
 
+// the error is reported here: it does not stay behind for the thread's next check
 #define OP_HIP(x, what)                                                             \
   do {                                                                              \
     hipError_t e_ = (x);                                                            \
-    if (e_ != hipSuccess)                                                           \
+    if (e_ != hipSuccess) {                                                         \
+      (void)hipGetLastError();                                                      \
       return g2v::op_fail(G2V_EHIP, "%s: %s", (what), hipGetErrorString(e_));       \
+    }                                                                               \
   } while (0)
