@@ -121,7 +121,8 @@ void check_scale(double scale) {
 
 // a whole number as Python gives it: int, numpy integer, 3.0
 int64_t whole(py::handle h, const char* name) {
-  const double d = py::cast<double>(py::float_(py::reinterpret_borrow<py::object>(h)));
+  const double d = PyFloat_AsDouble(h.ptr());  // a number: no text that holds one
+  if (PyErr_Occurred()) throw py::error_already_set();
   if (d != std::floor(d) || std::fabs(d) > 9e15)
     refuse(std::string(name) + " must be a whole number, not " + std::string(py::str(h)));
   return (int64_t)d;

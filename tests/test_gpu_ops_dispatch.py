@@ -228,3 +228,21 @@ def test_the_gradient_refuses_a_dy_that_requires_one():
     assert torch.equal(ops.embedding_lookup_grad(dy.detach(), ids, V), want)
     with pytest.raises(RuntimeError, match="once, not twice"):  # past the Python entry
         torch.ops.g2v.embedding_lookup_grad(dy, ids, V, 1.0, -1, torch.float32).sum().backward()
+
+
+def test_whole_numbers_are_numbers():
+    import numpy as np
+    w, ids, dy = inputs(14)
+    want = ops.embedding_lookup_grad(dy, ids, V, padding_idx=3)
+    for three in (3, 3.0, np.int32(3), np.float32(3), torch.tensor(3)):
+        for v in (V, float(V), np.int64(V)):
+            assert torch.equal(ops.embedding_lookup_grad(dy, ids, v, padding_idx=three), want)
+    for bad in ("3", b"3", [3], None):
+        with pytest.raises(TypeError):
+            ops.embedding_lookup_grad(dy, ids, bad)
+        if bad is not None:
+            with pytest.raises(TypeError):
+                ops.embedding_lookup(w, ids, padding_idx=bad)
+    for bad in (float("nan"), float("inf"), 10**30, 2.5):
+        with pytest.raises(ValueError, match="whole"):
+            ops.embedding_lookup_grad(dy, ids, bad)
