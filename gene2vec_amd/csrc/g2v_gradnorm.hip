@@ -8,8 +8,8 @@
 // The squares are formed and added in fp64: an fp32 sum would overflow from
 // elements of 1.8e19 on and lose the small tensors beside the large ones, and
 // gfx950 adds fp64 far faster than memory delivers the elements.  Memory bound:
-// 10^9 bf16 elements in 48 tensors 338 us (5.9 TB/s), clipping 3 * 10^8 elements
-// of two types in 600 tensors 593 us (1 GB read twice and written).  No atomics:
+// 10^9 bf16 elements in 48 tensors 314 us (6.4 TB/s), clipping 3 * 10^8 elements
+// of two types in 600 tensors 586 us (1 GB read twice and written).  No atomics:
 // every workgroup writes one partial sum, and they are added in a fixed order,
 // so the same gradients give the same bits.
 //
@@ -29,7 +29,12 @@ using g2v::f16;
 
 constexpr int kThreads = 256;
 constexpr int kTensors = 128;       // per launch: 3.7 KB of arguments
-constexpr int kMaxPartials = 2048;  // workgroups: 8 per CU, all resident
+constexpr int kMaxPartials = 2048;  // workgroups: 8 per CU
+// all of them resident: 8 waves a SIMD, so at most 64 registers.  At the 66 and 73
+// that the compiler takes unasked only 7 or 6 of a CU's 8 fit, and the rest of
+// the equal shares begin when the first have ended: the norm of 10^9 bf16
+// elements 314 us against 339, clipping 3 * 10^8 in 600 tensors 586 against 590
+constexpr int kWaves = 8;
 constexpr int64_t kChunk = 8192;    // elements a workgroup takes at a time
 constexpr int kAlign = 64;          // bytes: where a tensor's chunks begin
 
@@ -159,7 +164,7 @@ __device__ __forceinline__ void for_elements(const A& a, F f) {
 }
 
 template <bool NT, class A>
-__global__ __launch_bounds__(kThreads) void k_square_sum(A a, double* __restrict__ partial) {
+__global__ __launch_bounds__(kThreads, kWaves) void k_square_sum(A a, double* __restrict__ partial) {
   double s0 = 0.0, s1 = 0.0;
   for_elements<NT>(a, [&](int, auto, int64_t, auto& x) {
     constexpr int N = sizeof x / sizeof x[0];
@@ -192,7 +197,7 @@ __global__ __launch_bounds__(kThreads) void k_norm(const double* __restrict__ pa
 // the norm's pass leaves them the gradients: of 400 MB fp32 clipped to another
 // buffer 194 us, 250 with ordinary accesses, 217 with the norm's pass past them.
 template <class A>
-__global__ __launch_bounds__(kThreads) void k_clip(A a, const double* __restrict__ partial, int np,
+__global__ __launch_bounds__(kThreads, kWaves) void k_clip(A a, const double* __restrict__ partial, int np,
                                                    double clip, bool in_place,
                                                    float* __restrict__ norm) {
   const double nrm = sqrt(sum_partials(partial, np));

@@ -60,3 +60,20 @@ def test_kernel_hash_covers_the_flags(monkeypatch):
     # counters of the kernels with packed arithmetic are of another build
     old = json.load(open(os.path.join(B.ROOT, "profiles", "r06", "traffic_r06.json")))
     assert old["kernel_src_sha16"] != here
+
+
+def test_norm_and_clip_workgroups_are_all_resident(tmp_path):
+    """their grids are sized to 8 waves a SIMD"""
+    src = "g2v_gradnorm.hip"
+    cmd = [B.hipcc(), *B.COMPILE_FLAGS, *B.unit_flags(src), "-I", os.path.join(B.ROOT, "include"),
+           "-I", B.CSRC, "-Rpass-analysis=kernel-resource-usage", "--cuda-device-only", "-c",
+           os.path.join(B.CSRC, src), "-o", str(tmp_path / "x.o")]
+    r = subprocess.run(cmd, capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stderr[-3000:]
+    found = 0
+    for part in r.stderr.split("Function Name: ")[1:]:
+        if re.match(r"\S*(k_square_sum|k_clip)", part):
+            found += 1
+            assert re.search(r"Occupancy \[waves/SIMD\]: 8\b", part), part
+            assert re.search(r"VGPRs Spill: 0\b", part), part
+    assert found == 6
