@@ -663,12 +663,23 @@ struct Plan {
 
 Plan plan(int64_t n, int64_t V, int64_t D) {
   Plan p{};
-  // short pieces spread a frequent row over more groups, long ones leave less
-  // to join: the gradient of 65,536 tokens of 24,447 x 200 fp32 takes 42 us at
-  // 64, 42 at 32, 46 at 128; of 262,147 of 60,000 x 512 127 us at 64, 122 at 128,
-  // 119 at 256.  A few hundred tokens are not cut at all, which saves a launch of
-  // three (11 us instead of 12).
-  p.log2L = n <= 256 ? 8 : n <= 65536 ? 6 : n <= 262144 ? 7 : 8;
+  // Short pieces spread a frequent row over more groups, long ones leave less to
+  // join: the more elements, the more pieces there are to fill the card with, and
+  // the longer they may be.  Microseconds of the gradient at L = 64 / 128 / 256,
+  // rows by Zipf's law and (in brackets) two rows only:
+  //   elements  64 columns bf16         200 fp32                512 bf16
+  //   2^20      24 / 27 / 38            18 / 21 / 24            23 / 23 / 25
+  //             (27 / 30 / 40)          (20 / 23 / 30)          (23 / 25 / 34)
+  //   2^23      43 / 50 / 64            36 / 39 / 48            29 / 30 / 42
+  //             (48 / 48 / 55)          (42 / 44 / 51)          (33 / 32 / 40)
+  //   2^25.5    74 / 71 / 81            64 / 64 / 69            57 / 55 / 65
+  //             (106 / 87 / 88)         (73 / 65 / 64)          (67 / 58 / 66)
+  //   2^27      119 / 109 / 109         197 / 186 / 186         106 / 97 / 98
+  //             (187 / 147 / 129)       (274 / 222 / 196)       (129 / 101 / 100)
+  // Up to 256 tokens are not cut at all, which saves a launch of three (200
+  // tokens: 11 us instead of 13; at 300 the longest run costs as much).
+  const int64_t elements = n * D;
+  p.log2L = n <= 256 ? 8 : elements < (int64_t)1 << 24 ? 6 : elements < (int64_t)1 << 26 ? 7 : 8;
   p.chunks = (n + ((int64_t)1 << p.log2L) - 1) >> p.log2L;
   p.slots = n > (int64_t)1 << p.log2L ? 2 * p.chunks : 0;
   if (n > kScanTokens || (n > 0 && V > kScanRows)) {
