@@ -99,7 +99,9 @@ constexpr int kBuckets = 256;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWaves = kSortThreads / 64;
 constexpr int kKeys = 1024;         // rows a bucket counts at a time (64 KB of LDS)
-constexpr int kListBits = 10;       // tokens a wave lists: 2^10 (4 KB of LDS)
+constexpr int kListBits = 10;       // tokens a wave lists: 2^10 (64 KB of LDS in all, what
+                                    // the counts leave room for; 20,000 tokens the other
+                                    // way take 31 us where 16,384 take 22)
 constexpr int kScanTokens = kSortWaves << kListBits;
 constexpr int64_t kScanRows = (int64_t)kBuckets << (32 - kListBits);  // a list entry's row
 constexpr int kTileTokens = 1024;   // 65,536 tokens: 42 us, 45 with 4096
@@ -523,9 +525,10 @@ __device__ __forceinline__ void sum_rows(const TY* __restrict__ dy, int64_t ld,
 // times G vectors of a row, so that the many rows without a token are written by
 // fewer groups that live long enough to pay for reading the count: the gradient
 // of 16,384 tokens of 131,072 x 4,096 bf16 takes 272 us at 1, 247 at 2, 257 at 4;
-// with ordinary stores, not past the caches, 268 at 2.  218 of the 247 are this
-// kernel (1.2 GB, 5.5 TB/s; 160 where dy is still in the Infinity Cache, which is
-// what filling a tensor of that size takes).
+// with ordinary stores, not past the caches, 268 at 2 (all with pieces of 64
+// tokens; 237 with the 256 of today).  221 us are this kernel (1.2 GB, 5.4 TB/s;
+// 160 where dy is still in the Infinity Cache, which is what filling a tensor of
+// that size takes).
 //
 // A longer run is cut at every L-th of its tokens into pieces, first in the grid
 // as they take longest and G vectors a group; their sums go to part.  Pieces are

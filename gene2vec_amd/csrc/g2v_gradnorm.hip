@@ -195,7 +195,7 @@ __global__ __launch_bounds__(kThreads) void k_norm(const double* __restrict__ pa
 // factor everywhere): 16 KB from the L2 instead of a launch in between.  What
 // is read here for the last time and what is written go past the caches, and
 // the norm's pass leaves them the gradients: of 400 MB fp32 clipped to another
-// buffer 194 us, 250 with ordinary accesses, 217 with the norm's pass past them.
+// buffer 190 us, 243 with ordinary accesses, 211 with the norm's pass past them.
 template <class A>
 __global__ __launch_bounds__(kThreads, kWaves) void k_clip(A a, const double* __restrict__ partial, int np,
                                                    double clip, bool in_place,
@@ -369,8 +369,8 @@ extern "C" int g2v_global_norm(int device, const void* const* tensors, const int
   const hipStream_t st = static_cast<hipStream_t>(stream);
   double* partial = static_cast<double*>(workspace);
   // beyond the Infinity Cache's 256 MB nothing stays for the next reader, and
-  // loads past the caches are faster (1 GB of fp32: 167 us against 190); what
-  // fits may still lie there (200 MB: 38 us against 35)
+  // loads past the caches are faster (1 GB of fp32: 149 us against 170, 400 MB 63
+  // against 72); what fits may still lie there (250 MB: 41.5 us against 40)
   double bytes = 0.0;
   for (int64_t t = 0; t < n; ++t) bytes += (double)(numel[t] * g2v::type_bytes(types[t]));
   const bool large = bytes > 256e6;

@@ -6,6 +6,9 @@
     global_norm            the 2-norm over a list of gradients
     clip_by_global_norm    the list scaled down to a norm; ``_`` at the end: in place
 
+They are torch operators too (``torch.ops.g2v``, which this module registers):
+tracers, functional transforms and dispatch modes see them.
+
 They run in ``libg2v.so`` on the tensors' own device and on torch's current
 stream there, without synchronising; there is no CPU fallback.  Tensors that
 another stream made are the caller's to wait for, and to ``record_stream``, as
