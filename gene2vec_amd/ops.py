@@ -16,13 +16,16 @@ with any torch operator.  Workspaces come from torch's allocator in each call,
 so calls on several streams do not share any, and a call captured into a
 ``torch.cuda.graph`` keeps its own in the graph's pool.  The same inputs give
 the same bits.  Tensors and values that do not fit raise ``ValueError``
-before anything runs, the library's own errors ``_native.G2VError``.
+(``TypeError``: what is no number) before anything runs, the library's own
+errors ``_native.G2VError``.
 
 A lookup in a table that requires its gradient is captured only while no graph
 of that leaf, or of a leaf that the table was computed from, lives from the
 default stream (``del`` the loss of earlier steps): torch accumulates on the
 stream that graph was built on, and the default stream ends a capture, so the
-call raises ``ValueError`` then.
+call raises ``ValueError`` then.  A backward pass is captured together with its
+lookup: one that was looked up before the capture, on another stream, is torch's
+to run there, with the same end.
 """
 from __future__ import annotations
 
